@@ -1413,7 +1413,7 @@ def host_pack_baseline(dense_np, budget_s=10.0, fp8=False):
             _, _, meta = O.ref_compress_a(a, M, K)
             O.ref_reorder_metadata(meta, M, K)
         else:
-            _, meta = O.compress_a(a, M, K)
+            _, _, meta = O.compress_a(a, M, K)
             O.reorder_metadata(meta, M, K)
 
     probe = 64
