@@ -370,11 +370,38 @@ __device__ __forceinline__ bool pack_group8(uint32_t w, uint32_t prune_top, uint
     return ((0x0117u >> z) & 1u) == 0;
 }
 
+// The same for int8 values: magnitudes 0 .. 128 (ties prefer the lower
+// position), and only the byte 0 is a zero.
+__device__ __forceinline__ bool pack_group_i8(uint32_t w, bool prune, uint32_t* pair, uint32_t* idx) {
+    if (prune) {
+        const uint32_t a = __vabs4(w);  // -128 -> 0x80: an unsigned magnitude
+        uint32_t keep = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            int ahead = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t ai = (a >> (8 * i)) & 0xffu, aj = (a >> (8 * j)) & 0xffu;
+                if (j != i) ahead += aj > ai || (aj == ai && j < i);
+            }
+            keep |= ahead < 2 ? 0xffu << (8 * i) : 0u;
+        }
+        w &= keep;
+    }
+    const uint32_t z = ((w & 0xffu) == 0 ? 1u : 0u) | ((w & 0xff00u) == 0 ? 2u : 0u) |
+                       ((w & 0xff0000u) == 0 ? 4u : 0u) | ((w & 0xff000000u) == 0 ? 8u : 0u);
+    const uint32_t id = (uint32_t)(0xECD4E894ECD4E444ull >> (4 * z)) & 0xfu;  // as in pack_group8
+    *pair = __byte_perm(w, 0, (id & 3u) | ((id >> 2) << 4) | 0x4400u);
+    *idx = id;
+    return ((0x0117u >> z) & 1u) == 0;
+}
+
 // One CTA: kPackBands 16-row bands x 512 bytes of K (16 blocks of 32 K), the
 // 16-bit kernel's tile geometry in bytes.  Thread t handles row t % 16 of
 // block t / 16 in every band: 32 bytes in, 16 value bytes and 4 metadata
-// bytes out.
-__global__ void __launch_bounds__(kPackThreads) pack_a_fp8_kernel(const uint8_t* __restrict__ dense, int M, int K,
+// bytes out.  I8: int8 values (prune_top: 0 no prune, else prune).
+template <bool I8>
+__global__ void __launch_bounds__(kPackThreads) pack_a_bytes_kernel(const uint8_t* __restrict__ dense, int M, int K,
                                                                   uint32_t prune_top, uint8_t* __restrict__ vals,
                                                                   uint8_t* __restrict__ meta, int* bad_blocks) {
     __shared__ __align__(16) uint8_t tile[kPackBands * 16 * kTilePitch * 2];
@@ -422,7 +449,7 @@ __global__ void __launch_bounds__(kPackThreads) pack_a_fp8_kernel(const uint8_t*
         bool ok = true;
         // Row fast path (prune on, no NaN in the row's 32 bytes, both kept
         // magnitudes of every group non-zero); otherwise per group.
-        bool fast = prune_top != 0;
+        bool fast = !I8 && prune_top != 0;
         uint32_t top4[4], sec4[4];
         if (fast) {
             const uint32_t add = (0x7fu - prune_top) * 0x01010101u;
@@ -447,7 +474,7 @@ __global__ void __launch_bounds__(kPackThreads) pack_a_fp8_kernel(const uint8_t*
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 uint32_t idx;
-                ok &= pack_group8(w[k], prune_top, &pr[k], &idx);
+                ok &= I8 ? pack_group_i8(w[k], prune_top != 0, &pr[k], &idx) : pack_group8(w[k], prune_top, &pr[k], &idx);
                 md |= idx << (4 * k);
             }
             out = make_uint4(pr[0] | (pr[1] << 16), pr[2] | (pr[3] << 16), pr[4] | (pr[5] << 16), pr[6] | (pr[7] << 16));
@@ -548,22 +575,40 @@ extern "C" cudaError_t spmm24_pack_a_device(cudaStream_t stream, const void* den
                       static_cast<uint16_t*>(values_out), meta_out, bad_blocks);
 }
 
-extern "C" cudaError_t spmm24_pack_a_fp8_device(cudaStream_t stream, const void* dense_a, int M, int K, int prune,
-                                                void* values_out, void* meta_out, int* bad_blocks) {
-    using namespace spmm24;
-    clear_last_error();
+namespace spmm24 {
+namespace {
+template <bool I8>
+cudaError_t pack_a_bytes(cudaStream_t stream, const void* dense_a, int M, int K, uint32_t prune_top, void* values_out,
+                         void* meta_out, int* bad_blocks) {
     if (!dense_a || !values_out || !meta_out) return record_invalid("null pointer");
     if (M <= 0 || K <= 0 || M % 16 || K % 128) return record_invalid("M must be a multiple of 16 and K of 128");
     if (misaligned16(dense_a) || misaligned16(values_out) || misaligned16(meta_out))
         return record_invalid("dense A, values and metadata must be 16-byte aligned");
     if (reinterpret_cast<uintptr_t>(bad_blocks) & 3u) return record_invalid("bad_blocks must be 4-byte aligned");
-    if (prune < 0 || prune > 2) return record_invalid("prune: 0 none, 1 E4M3, 2 E5M2");
     const int nbc = K / 32;
     dim3 grid((unsigned)((nbc + kTileBlocks - 1) / kTileBlocks), (unsigned)((M / 16 + kPackBands - 1) / kPackBands));
     if (grid.y > 65535) return record_invalid("M too large");
-    const uint32_t top = prune == 1 ? 0x7eu : prune == 2 ? 0x7cu : 0u;
-    return launch_pdl(pack_a_fp8_kernel, grid, stream, static_cast<const uint8_t*>(dense_a), M, K, top,
+    return launch_pdl(pack_a_bytes_kernel<I8>, grid, stream, static_cast<const uint8_t*>(dense_a), M, K, prune_top,
                       static_cast<uint8_t*>(values_out), static_cast<uint8_t*>(meta_out), bad_blocks);
+}
+}  // namespace
+}  // namespace spmm24
+
+extern "C" cudaError_t spmm24_pack_a_fp8_device(cudaStream_t stream, const void* dense_a, int M, int K, int prune,
+                                                void* values_out, void* meta_out, int* bad_blocks) {
+    using namespace spmm24;
+    clear_last_error();
+    if (prune < 0 || prune > 2) return record_invalid("prune: 0 none, 1 E4M3, 2 E5M2");
+    const uint32_t top = prune == 1 ? 0x7eu : prune == 2 ? 0x7cu : 0u;
+    return pack_a_bytes<false>(stream, dense_a, M, K, top, values_out, meta_out, bad_blocks);
+}
+
+extern "C" cudaError_t spmm24_pack_a_int8_device(cudaStream_t stream, const void* dense_a, int M, int K, int prune,
+                                                 void* values_out, void* meta_out, int* bad_blocks) {
+    using namespace spmm24;
+    clear_last_error();
+    if (prune < 0 || prune > 1) return record_invalid("prune: 0 none, 1 by magnitude");
+    return pack_a_bytes<true>(stream, dense_a, M, K, (uint32_t)prune, values_out, meta_out, bad_blocks);
 }
 
 namespace spmm24 {

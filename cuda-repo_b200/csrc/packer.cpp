@@ -215,7 +215,12 @@ extern "C" int spmm24_prune_2of4_fp8(uint8_t* a, int M, int K, int fmt) { return
 // Metadata: band b, 128-K group g, row r -> 16 bytes at ((b*K/128 + g)*16 +
 // r)*16, nibble c = group of four at K 128g + 4c (i0 | i1 << 2, i0 < i1).
 // Compress rule of the 16-bit packer (test/utils.h:124-146) on bytes.
-extern "C" int spmm24_compress_a_fp8(const uint8_t* dense, int M, int K, uint8_t* vals, uint8_t* meta) {
+// MASK: the bits that a zero has clear (0x7f: fp8, whose zeros are +0 and
+// -0; 0xff: int8).
+namespace {
+
+template <uint32_t MASK>
+int compress_bytes(const uint8_t* dense, int M, int K, uint8_t* vals, uint8_t* meta) {
     if (!dense || !vals || !meta || M <= 0 || K <= 0 || M % 16 || K % 128) return -1;
     const int blocks = K / 32, groups = K / 128;
     std::vector<char> bad((size_t)(M / 16), 0);
@@ -232,7 +237,7 @@ extern "C" int spmm24_compress_a_fp8(const uint8_t* dense, int M, int K, uint8_t
                         uint8_t* dst = vals + (((size_t)band * blocks + k / 32) * 16 + r) * 16 + (k % 32) / 2;
                         for (int o = 0; o < 4; ++o) {
                             const uint8_t x = src[k + o];
-                            if (zeros < 2 && (x & 0x7fu) == 0) {
+                            if (zeros < 2 && (x & MASK) == 0) {
                                 ++zeros;
                                 continue;
                             }
@@ -253,6 +258,38 @@ extern "C" int spmm24_compress_a_fp8(const uint8_t* dense, int M, int K, uint8_t
     for (char b : bad)
         if (b) return -2;
     return (int)((size_t)M * K / 2);
+}
+
+}  // namespace
+
+extern "C" int spmm24_compress_a_fp8(const uint8_t* dense, int M, int K, uint8_t* vals, uint8_t* meta) {
+    return compress_bytes<0x7fu>(dense, M, K, vals, meta);
+}
+
+// ------------------------------------------------------------------ int8
+extern "C" int spmm24_prune_2of4_int8(int8_t* a, int M, int K) {
+    if (!a || M <= 0 || K <= 0 || K % 4) return -1;
+    parallel_for(M, K, [&](int m0, int m1) {
+        for (int m = m0; m < m1; ++m) {
+            int8_t* row = a + (size_t)m * K;
+            for (int g = 0; g < K; g += 4) {
+                int v[4];
+                for (int i = 0; i < 4; ++i) v[i] = std::abs((int)row[g + i]);
+                int k0 = 0, k1 = -1;
+                for (int i = 1; i < 4; ++i)
+                    if (v[i] > v[k0]) k0 = i;
+                for (int i = 0; i < 4; ++i)
+                    if (i != k0 && (k1 < 0 || v[i] > v[k1])) k1 = i;
+                for (int i = 0; i < 4; ++i)
+                    if (i != k0 && i != k1) row[g + i] = 0;
+            }
+        }
+    });
+    return 0;
+}
+
+extern "C" int spmm24_compress_a_int8(const int8_t* dense, int M, int K, uint8_t* vals, uint8_t* meta) {
+    return compress_bytes<0xffu>(reinterpret_cast<const uint8_t*>(dense), M, K, vals, meta);
 }
 
 // ------------------------------------------------- C++ reference drop-ins

@@ -232,6 +232,17 @@ __device__ __forceinline__ void mma_sp_f8(uint32_t d_tmem, uint64_t a_desc, uint
         : "memory");
 }
 
+// The int8 form (kind::i8): s32 accumulators, wrapping sums.
+__device__ __forceinline__ void mma_sp_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t meta_tmem,
+                                          uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.sp.cta_group::1.kind::i8 [%0], %1, %2, [%3], %4, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(meta_tmem), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
 // 128 lanes x 128 bits from shared memory (canonical no-swizzle K-major
 // layout: 8-row core matrices of 16-byte rows) into TMEM lanes 0..127,
 // four consecutive 32-bit columns.
@@ -274,6 +285,15 @@ __device__ __forceinline__ void mma_sp_f8_pair(uint32_t d_tmem, uint64_t a_desc,
         "{\n\t.reg .pred p;\n\t"
         "setp.ne.b32 p, %5, 0;\n\t"
         "tcgen05.mma.sp.cta_group::2.kind::f8f6f4 [%0], %1, %2, [%3], %4, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(meta_tmem), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void mma_sp_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t meta_tmem,
+                                               uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.sp.cta_group::2.kind::i8 [%0], %1, %2, [%3], %4, p;\n\t}" ::"r"(d_tmem),
         "l"(a_desc), "l"(b_desc), "r"(meta_tmem), "r"(idesc), "r"(accumulate)
         : "memory");
 }

@@ -171,6 +171,8 @@ constexpr int kPair2Stages = 3;
 using Pair2C = Pair2Cfg<kPair2Stages>;
 using Pair2C8 = Pair2Cfg<kPair2Stages, true>;
 using PairC8 = PairCfg<kPairStages, true>;
+using PairCI8 = PairCfg<kPairStages, true, 128, true>;
+using Pair2CI8 = Pair2Cfg<kPair2Stages, true, true>;
 // Stream-K variants: the scratch-array kernel of spmm24_launch_noalloc.
 using SV16 = StreamKVariant<16, 8>;
 using SV32 = StreamKVariant<32, 8>;
@@ -351,7 +353,7 @@ Plan make_plan(int M, int N, int K, int split_k, int sms, bool allow_pair = true
     return p;
 }
 
-std::atomic<uint64_t> g_attr_done[96];  // per kernel variant: one bit per device
+std::atomic<uint64_t> g_attr_done[128];  // per kernel variant: one bit per device
 
 // The plain SpMM: fp16, row-major C, no epilogue work.
 bool epilogue_plain_fp16(const Epilogue& e) {
@@ -441,6 +443,20 @@ cudaError_t launch_cluster_fp8(const Plan& pl, cudaStream_t stream, int dev, boo
                          stream, (unsigned)pl.split, pdl, ta, tb, te, kp);
 }
 
+// The int8 instantiations (always the general epilogue).
+constexpr int kInt8Slot = 96;
+
+template <class V>
+cudaError_t launch_cluster_int8(const Plan& pl, cudaStream_t stream, int dev, bool pdl, const CUtensorMap& ta,
+                                const CUtensorMap& tb, const CUtensorMap& te, const ClusterParams& kp, int idx) {
+    using CI8 = ClusterCfg<V::kTileN, V::kStages, true, true>;
+    auto kern = spmm24_cluster_kernel<V::kTileN, V::kStages, true, true, true>;
+    cudaError_t e = prepare(kern, CI8::SMEM_ALLOC, dev, kInt8Slot + idx);
+    if (e != cudaSuccess) return e;
+    return launch_kernel(kern, dim3((unsigned)pl.split, (unsigned)pl.n_tiles, (unsigned)pl.m_tiles), CI8::SMEM_ALLOC,
+                         stream, (unsigned)pl.split, pdl, ta, tb, te, kp);
+}
+
 template <class V>
 cudaError_t launch_streamk(const Plan& pl, cudaStream_t stream, int dev, bool pdl, const CUtensorMap& ta,
                            const CUtensorMap& tb, const CUtensorMap& te, const StreamKParams& kp, int idx) {
@@ -462,15 +478,27 @@ cudaError_t launch_pair_v(const Plan& pl, cudaStream_t stream, int dev, bool pdl
                          pdl, ta, tb, te, kp, kPairThreads);
 }
 
-template <bool KSPLIT>
+template <bool KSPLIT, bool I8>
 cudaError_t launch_pair_fp8(const Plan& pl, cudaStream_t stream, int dev, bool pdl, const CUtensorMap& ta,
                             const CUtensorMap& tb, const CUtensorMap& te, const PairParams& kp) {
-    auto kern = spmm24_pair_kernel<kPairStages, true, KSPLIT, true>;
-    cudaError_t e = prepare(kern, PairC8::SMEM_ALLOC, dev, kFp8Slot + (KSPLIT ? 12 : 11));
+    constexpr int SMEM = PairCfg<kPairStages, true, 128, I8>::SMEM_ALLOC;
+    auto kern = spmm24_pair_kernel<kPairStages, true, KSPLIT, true, 128, I8>;
+    cudaError_t e = prepare(kern, SMEM, dev, (I8 ? kInt8Slot : kFp8Slot) + (KSPLIT ? 12 : 11));
     if (e != cudaSuccess) return e;
     const unsigned cl = KSPLIT ? 4u : 2u;
-    return launch_kernel(kern, dim3(cl, (unsigned)pl.n_tiles, (unsigned)pl.m_tiles), PairC8::SMEM_ALLOC, stream, cl,
-                         pdl, ta, tb, te, kp, kPairThreads);
+    return launch_kernel(kern, dim3(cl, (unsigned)pl.n_tiles, (unsigned)pl.m_tiles), SMEM, stream, cl, pdl, ta, tb, te,
+                         kp, kPairThreads);
+}
+
+template <bool I8>
+cudaError_t launch_pair2_fp8(const Plan& pl, cudaStream_t stream, int dev, bool pdl, const CUtensorMap& ta,
+                             const CUtensorMap& tb, const CUtensorMap& te, const PairParams& kp) {
+    constexpr int SMEM = Pair2Cfg<kPair2Stages, true, I8>::SMEM_ALLOC;
+    auto kern = spmm24_pair2_kernel<kPair2Stages, true, true, I8>;
+    cudaError_t e = prepare(kern, SMEM, dev, (I8 ? kInt8Slot : kFp8Slot) + 13);
+    if (e != cudaSuccess) return e;
+    return launch_kernel(kern, dim3(2u, (unsigned)pl.n_tiles, (unsigned)pl.m_tiles), SMEM, stream, 2u, pdl, ta, tb, te,
+                         kp, kPairThreads);
 }
 
 cudaError_t launch_pair2(const Plan& pl, cudaStream_t stream, int dev, bool pdl, const CUtensorMap& ta,
@@ -606,7 +634,7 @@ cudaError_t launch_impl(cudaStream_t stream, const void* A, const void* B, const
             pl.split = 1;
             pl.grid = 2 * pl.m_tiles * pl.n_tiles;
         }
-        PairParams kp;
+        PairParams kp{};
         kp.C = static_cast<uint16_t*>(C);
         kp.epi = epi;
         kp.M = M;
@@ -619,7 +647,7 @@ cudaError_t launch_impl(cudaStream_t stream, const void* A, const void* B, const
         if (pl.pair2) return launch_pair2(pl, stream, dev, pdl, ta, tb, te, kp);
         return launch_pair(pl, stream, dev, pdl, ta, tb, te, kp);
     }
-    ClusterParams kp;
+    ClusterParams kp{};
     kp.C = static_cast<uint16_t*>(C);
     kp.epi = epi;
     kp.M = M;
@@ -654,45 +682,56 @@ cudaError_t launch_impl(cudaStream_t stream, const void* A, const void* B, const
 // early CTAs), and 11008-row layers pick 3 either way.  Wide N takes the CTA
 // pair as for 16-bit operands (its stage is 256 K: K % 256), and the
 // two-M-half pair (512 x 240) when its waves cost less and the epilogue has
-// no residual (pair2_ok).
+// no residual (pair2_ok).  The int8 SpMM (i8) has the same formats, stages and
+// plans, but for the two-M-half pair's tile of 512 x 224.
 template <class V>
-int fp8_smem() {
-    return ClusterCfg<V::kTileN, V::kStages, true>::SMEM_ALLOC;
+int fp8_smem(bool i8) {
+    return i8 ? ClusterCfg<V::kTileN, V::kStages, true, true>::SMEM_ALLOC : ClusterCfg<V::kTileN, V::kStages, true>::SMEM_ALLOC;
 }
 
-Plan plan_fp8(int M, int N, int K, int split_k, int sms, bool pair2_ok) {
+Plan plan_fp8(int M, int N, int K, int split_k, int sms, bool pair2_ok, bool i8 = false) {
     const int Kh = K / 2;
     Plan pl = make_plan(M, N, Kh, split_k, sms, Kh % 128 == 0, 5, false, false);
     if (pl.path == Path::kPair) {
-        pl.smem = PairC8::SMEM_ALLOC;
+        pl.smem = i8 ? PairCI8::SMEM_ALLOC : PairC8::SMEM_ALLOC;
         if (pl.split == 1 && split_k <= 1 && pair2_ok)
-            maybe_pair2(pl, M, N, sms, Pair2C8::TILE_N, kPair2Stages, Pair2C8::SMEM_ALLOC);
+            maybe_pair2(pl, M, N, sms, i8 ? Pair2CI8::TILE_N : Pair2C8::TILE_N, kPair2Stages,
+                        i8 ? Pair2CI8::SMEM_ALLOC : Pair2C8::SMEM_ALLOC);
     } else if (pl.shallow) {
-        pl.smem = pl.tile_n == 16 ? fp8_smem<CV16s>() : fp8_smem<CV32s>();
+        pl.smem = pl.tile_n == 16 ? fp8_smem<CV16s>(i8) : fp8_smem<CV32s>(i8);
     } else {
         switch (pl.tile_n) {
-            case 16: pl.smem = fp8_smem<CV16>(); break;
-            case 32: pl.smem = fp8_smem<CV32>(); break;
-            case 64: pl.smem = fp8_smem<CV64>(); break;
-            case 128: pl.smem = fp8_smem<CV128>(); break;
-            default: pl.smem = fp8_smem<CV256>(); break;
+            case 16: pl.smem = fp8_smem<CV16>(i8); break;
+            case 32: pl.smem = fp8_smem<CV32>(i8); break;
+            case 64: pl.smem = fp8_smem<CV64>(i8); break;
+            case 128: pl.smem = fp8_smem<CV128>(i8); break;
+            default: pl.smem = fp8_smem<CV256>(i8); break;
         }
     }
     return pl;
 }
+
+// K of an int8 product: K / 2 kept products of at most 2^14 each fit in 31 bits.
+constexpr int kInt8MaxK = 262144 - 128;
+
+// fp8 operands, or (i8) int8 operands with a scale for each row of A
+// (w_scale) and of B (x_scale), either of which may be null.
 cudaError_t launch_fp8_impl(cudaStream_t stream, const void* A, const void* B, const void* E, void* C, int M, int N,
-                            int K, int split_k, unsigned flags, const spmm24_epilogue* user_epi) {
+                            int K, int split_k, unsigned flags, const spmm24_epilogue* user_epi, bool i8 = false,
+                            const float* w_scale = nullptr, const float* x_scale = nullptr) {
     g_last_error[0] = '\0';
     if (!A || !B || !E || !C) return invalid("null pointer");
     if (M <= 0 || N <= 0 || K <= 0) return invalid("M, N and K must be positive");
     if (M % 16) return invalid("M must be a multiple of 16");
-    if (K % 128) return invalid("fp8: K must be a multiple of 128");
+    if (K % 128) return invalid(i8 ? "int8: K must be a multiple of 128" : "fp8: K must be a multiple of 128");
+    if (i8 && K > kInt8MaxK) return invalid("int8: K must be below 262144 (32-bit sums)");
+    if (((uintptr_t)w_scale | (uintptr_t)x_scale) & 3u) return invalid("int8: the scales must be 4-byte aligned");
     if (split_k < 0) return invalid("split_k must be >= 0");
     if (((uintptr_t)A | (uintptr_t)B | (uintptr_t)E) & 15u) return invalid("A, B and metadata must be 16-byte aligned");
     if ((uintptr_t)C & 1u) return invalid("C must be 2-byte aligned");
     if ((long)M / kTileM >= 65535) return invalid("M too large");
-    if (flags & ~(unsigned)(SPMM24_STATIC_WEIGHTS | SPMM24_NO_PDL | SPMM24_BF16 | SPMM24_FP8_A_E5M2 |
-                            SPMM24_FP8_B_E5M2))
+    if (flags & ~(unsigned)(SPMM24_STATIC_WEIGHTS | SPMM24_NO_PDL | SPMM24_BF16 |
+                            (i8 ? 0 : SPMM24_FP8_A_E5M2 | SPMM24_FP8_B_E5M2)))
         return invalid("unknown flag");
     Epilogue epi;
     cudaError_t e = make_epilogue(user_epi, flags, C, &epi);
@@ -701,7 +740,7 @@ cudaError_t launch_fp8_impl(cudaStream_t stream, const void* A, const void* B, c
     e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     const int Kh = K / 2;  // the 16-bit-equivalent K of the A bytes
-    Plan pl = plan_fp8(M, N, K, split_k, sm_count(dev), !epi.residual);
+    Plan pl = plan_fp8(M, N, K, split_k, sm_count(dev), !epi.residual, i8);
     const bool pair = pl.path == Path::kPair;
 
     CUtensorMap ta, tb, te;
@@ -716,7 +755,8 @@ cudaError_t launch_fp8_impl(cudaStream_t stream, const void* A, const void* B, c
     {
         cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)N};
         cuuint64_t str[1] = {(cuuint64_t)K};
-        cuuint32_t box[2] = {128, (cuuint32_t)(!pair ? pl.tile_n : pl.pair2 ? Pair2C8::HALF_N : PairC8::HALF_N)};
+        const int half2 = i8 ? Pair2CI8::HALF_N : Pair2C8::HALF_N;
+        cuuint32_t box[2] = {128, (cuuint32_t)(!pair ? pl.tile_n : pl.pair2 ? half2 : PairC8::HALF_N)};
         if (!encode(&tb, 2, B, dims, str, box, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B))
             return invalid("TMA descriptor for B could not be encoded");
     }
@@ -736,7 +776,7 @@ cudaError_t launch_fp8_impl(cudaStream_t stream, const void* A, const void* B, c
             pl.split = 1;
             pl.grid = 2 * pl.m_tiles * pl.n_tiles;
         }
-        PairParams kp;
+        PairParams kp{};
         kp.C = static_cast<uint16_t*>(C);
         kp.epi = epi;
         kp.M = M;
@@ -746,17 +786,18 @@ cudaError_t launch_fp8_impl(cudaStream_t stream, const void* A, const void* B, c
         kp.weights_static = (flags & SPMM24_STATIC_WEIGHTS) ? 1 : 0;
         kp.split = pl.split;
         kp.mma_fmt = mma_fmt;
-        if (pl.pair2) {
-            auto kern = spmm24_pair2_kernel<kPair2Stages, true, true>;
-            e = prepare(kern, Pair2C8::SMEM_ALLOC, dev, kFp8Slot + 13);
-            if (e != cudaSuccess) return e;
-            return launch_kernel(kern, dim3(2u, (unsigned)pl.n_tiles, (unsigned)pl.m_tiles), Pair2C8::SMEM_ALLOC,
-                                 stream, 2u, pdl, ta, tb, te, kp, kPairThreads);
-        }
-        return pl.split == 2 ? launch_pair_fp8<true>(pl, stream, dev, pdl, ta, tb, te, kp)
-                             : launch_pair_fp8<false>(pl, stream, dev, pdl, ta, tb, te, kp);
+        kp.w_scale = w_scale;
+        kp.x_scale = x_scale;
+        if (pl.pair2)
+            return i8 ? launch_pair2_fp8<true>(pl, stream, dev, pdl, ta, tb, te, kp)
+                      : launch_pair2_fp8<false>(pl, stream, dev, pdl, ta, tb, te, kp);
+        if (i8)
+            return pl.split == 2 ? launch_pair_fp8<true, true>(pl, stream, dev, pdl, ta, tb, te, kp)
+                                 : launch_pair_fp8<false, true>(pl, stream, dev, pdl, ta, tb, te, kp);
+        return pl.split == 2 ? launch_pair_fp8<true, false>(pl, stream, dev, pdl, ta, tb, te, kp)
+                             : launch_pair_fp8<false, false>(pl, stream, dev, pdl, ta, tb, te, kp);
     }
-    ClusterParams kp;
+    ClusterParams kp{};
     kp.C = static_cast<uint16_t*>(C);
     kp.epi = epi;
     kp.M = M;
@@ -767,6 +808,21 @@ cudaError_t launch_fp8_impl(cudaStream_t stream, const void* A, const void* B, c
     kp.split = pl.split;
     kp.weights_static = (flags & SPMM24_STATIC_WEIGHTS) ? 1 : 0;
     kp.mma_fmt = mma_fmt;
+    kp.w_scale = w_scale;
+    kp.x_scale = x_scale;
+    if (i8) {
+        if (pl.shallow) {
+            if (pl.tile_n == 16) return launch_cluster_int8<CV16s>(pl, stream, dev, pdl, ta, tb, te, kp, 9);
+            return launch_cluster_int8<CV32s>(pl, stream, dev, pdl, ta, tb, te, kp, 10);
+        }
+        switch (pl.tile_n) {
+            case 16: return launch_cluster_int8<CV16>(pl, stream, dev, pdl, ta, tb, te, kp, 0);
+            case 32: return launch_cluster_int8<CV32>(pl, stream, dev, pdl, ta, tb, te, kp, 1);
+            case 64: return launch_cluster_int8<CV64>(pl, stream, dev, pdl, ta, tb, te, kp, 2);
+            case 128: return launch_cluster_int8<CV128>(pl, stream, dev, pdl, ta, tb, te, kp, 3);
+            default: return launch_cluster_int8<CV256>(pl, stream, dev, pdl, ta, tb, te, kp, 4);
+        }
+    }
     if (pl.shallow) {
         if (pl.tile_n == 16) return launch_cluster_fp8<CV16s>(pl, stream, dev, pdl, ta, tb, te, kp, 9);
         return launch_cluster_fp8<CV32s>(pl, stream, dev, pdl, ta, tb, te, kp, 10);
@@ -1368,6 +1424,14 @@ extern "C" cudaError_t spmm24_launch_fp8(cudaStream_t stream, const void* values
     return spmm24::launch_fp8_impl(stream, values, b_nk, metadata, c, M, N, K, split_k, flags, epilogue);
 }
 
+extern "C" cudaError_t spmm24_launch_int8(cudaStream_t stream, const void* values, const void* b_nk,
+                                          const void* metadata, void* c, int M, int N, int K, const float* w_scale,
+                                          const float* x_scale, int split_k, unsigned flags,
+                                          const spmm24_epilogue* epilogue) {
+    return spmm24::launch_fp8_impl(stream, values, b_nk, metadata, c, M, N, K, split_k, flags, epilogue, true, w_scale,
+                                   x_scale);
+}
+
 extern "C" cudaError_t spmm24_launch_gather(cudaStream_t stream, const void* compressed_a, const void* b_packed,
                                             const uint16_t* metadata, int M, int N, int K, int split_k, unsigned flags,
                                             const spmm24_gather* gather) {
@@ -1519,6 +1583,12 @@ extern "C" int spmm24_select_config(int M, int N, int K, int split_k, spmm24_con
 extern "C" int spmm24_select_config_fp8(int M, int N, int K, int split_k, spmm24_config* out) {
     if (!out || M <= 0 || N <= 0 || K <= 0 || M % 16 || K % 128 || split_k < 0) return -1;
     spmm24::fill_config(spmm24::plan_fp8(M, N, K, split_k, spmm24::current_sms(), true), 256, out);
+    return 0;
+}
+
+extern "C" int spmm24_select_config_int8(int M, int N, int K, int split_k, spmm24_config* out) {
+    if (!out || M <= 0 || N <= 0 || K <= 0 || M % 16 || K % 128 || K > spmm24::kInt8MaxK || split_k < 0) return -1;
+    spmm24::fill_config(spmm24::plan_fp8(M, N, K, split_k, spmm24::current_sms(), true, true), 256, out);
     return 0;
 }
 

@@ -196,6 +196,10 @@ __host__ __device__ constexpr uint32_t make_idesc_fp8() {
 }
 constexpr uint32_t kIdescFp8AE5M2 = 1u << 7;
 constexpr uint32_t kIdescFp8BE5M2 = 1u << 10;
+// int8 (kind::i8) shares the fp8 operand and metadata layouts: the fp8
+// descriptor with D = s32 in place of f32 and signed 8-bit A and B.
+constexpr uint32_t kIdescF32 = 1u << 4;
+constexpr uint32_t kIdescInt8 = (2u << 4) | (1u << 7) | (1u << 10);
 
 // Metadata copies + the four fp8 sparse MMAs of one stage (single thread).
 // Metadata: each 128-K group is 128 rows x 16 bytes, one tcgen05.cp into
@@ -203,10 +207,11 @@ constexpr uint32_t kIdescFp8BE5M2 = 1u << 10;
 // takes 32-K blocks 2j, 2j+1 (K-major core matrices, 2048 B apart along K,
 // 128 B apart along M).  B: MMA j takes bytes 64 (j % 2) .. + 63 of every
 // row of the 128-byte swizzled half j / 2 (N_TILE rows of 128 B).
-template <class C_, int N_TILE>
+// I8: int8 operands in the same layouts (fmt is then unused).
+template <class C_, int N_TILE, bool I8 = false>
 __device__ __forceinline__ void mma_stage_fp8(uint32_t st_addr, uint32_t meta_col, uint32_t d_tmem,
                                               uint32_t& accumulate, uint32_t fmt) {
-    const uint32_t idesc = make_idesc_fp8<N_TILE>() | fmt;
+    const uint32_t idesc = I8 ? (make_idesc_fp8<N_TILE>() & ~kIdescF32) | kIdescInt8 : make_idesc_fp8<N_TILE>() | fmt;
     const uint32_t stB = st_addr + C_::A_BYTES;
     const uint32_t stE = stB + C_::B_BYTES;
     ptx::tmem_cp_128x128b(meta_col, smem_desc(stE, 0, 128));
@@ -215,7 +220,8 @@ __device__ __forceinline__ void mma_stage_fp8(uint32_t st_addr, uint32_t meta_co
     for (int j = 0; j < 4; ++j) {
         const uint64_t adesc = smem_desc(st_addr + j * 4096, 2048, 128);
         const uint64_t bdesc = smem_desc_sw128(stB + (j >> 1) * (C_::B_BYTES / 2) + (j & 1) * 64);
-        ptx::mma_sp_f8(d_tmem, adesc, bdesc, meta_col + 2 * j, idesc, accumulate);
+        if constexpr (I8) ptx::mma_sp_i8(d_tmem, adesc, bdesc, meta_col + 2 * j, idesc, accumulate);
+        else ptx::mma_sp_f8(d_tmem, adesc, bdesc, meta_col + 2 * j, idesc, accumulate);
         accumulate = 1;
     }
 }
@@ -288,6 +294,13 @@ __device__ __forceinline__ uint16_t f32_to_elem(float v, int bf16) {
     }
     const __half h = __float2half_rn(v);
     return static_cast<__half_raw>(h).x;
+}
+
+// int8 products: the exact s32 sum, scaled by its output row's and column's
+// scale.  Above 2^24 the conversion rounds the sum to 24 bits, relative
+// 2^-24, far below the 16-bit output's half ulp.
+__device__ __forceinline__ float int8_value(int acc, float w_scale, float x_scale) {
+    return (float)acc * w_scale * x_scale;
 }
 
 // Hardware tanh approximation (tanh.approx.f32: relative error about 2^-11,

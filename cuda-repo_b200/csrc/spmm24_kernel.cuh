@@ -39,7 +39,11 @@
 // row-major SpMM, and EPI (alpha, bias, activation, residual, bf16, packed
 // output, fused all-gather), kept apart because the epilogue of every tile
 // is on the critical path.  All but stream-K also come in an FP8 form (OCP
-// E4M3 / E5M2 operands, tcgen05.mma.sp kind::f8f6f4, stages of 256 K).
+// E4M3 / E5M2 operands, tcgen05.mma.sp kind::f8f6f4, stages of 256 K), and
+// in an I8 form on top of it: int8 operands in the same layouts, kind::i8,
+// s32 accumulators (K splits are added as integers, so the sum is exact and
+// every split gives the same bits), scaled per output row and column before
+// the general epilogue.
 //
 // Roles (192 threads; the pair kernel 256):
 //   warp 0     TMA producer (lane 0)
@@ -73,6 +77,8 @@ struct ClusterParams {
     int split;         // CTAs per cluster along K
     int weights_static;
     uint32_t mma_fmt;  // fp8 kernel: operand-format bits of the instruction descriptor
+    const float* w_scale;  // int8 kernel: a scale for each output row (null: 1)
+    const float* x_scale;  // int8 kernel: a scale for each output column (null: 1)
     Epilogue epi;
     SPMM24_TRACE_FIELD
 };
@@ -84,6 +90,8 @@ struct PairParams {
     int weights_static;
     int split;         // pairs per cluster along K (1 or 2)
     uint32_t mma_fmt;  // fp8 kernel: operand-format bits of the instruction descriptor
+    const float* w_scale;  // int8 kernel: a scale for each output row (null: 1)
+    const float* x_scale;  // int8 kernel: a scale for each output column (null: 1)
     Epilogue epi;
     SPMM24_TRACE_FIELD
 };
@@ -103,7 +111,7 @@ struct StreamKParams {
 };
 
 // -------------------------------------------------------------------------
-template <int N_TILE, int STAGES, bool FP8 = false>
+template <int N_TILE, int STAGES, bool FP8 = false, bool I8 = false>
 struct ClusterCfg : Cfg<N_TILE, STAGES, 1, FP8> {
     using B_ = Cfg<N_TILE, STAGES, 1, FP8>;
     static constexpr int RED_PITCH = N_TILE + 4;  // floats per row of the reduction buffer
@@ -120,8 +128,11 @@ struct ClusterCfg : Cfg<N_TILE, STAGES, 1, FP8> {
     static constexpr int BIAS_OFFSET = HOLDER_OFFSET + 16;  // the owner rows' bias, prefetched (EPI)
     // Narrow tiles: the owner rows' residual, prefetched (EPI, 16-byte layouts).
     static constexpr int RES_OFFSET = BIAS_OFFSET + kTileM * 4;
-    static constexpr int RES_BYTES = N_TILE <= 32 ? kTileM * N_TILE * 2 : 0;
-    static constexpr int SMEM_BYTES = RES_OFFSET + RES_BYTES;
+    // int8: the owner rows' and the tile columns' scales take its place (two
+    // CTAs still fit on one SM with the shallow ring).
+    static constexpr int RES_BYTES = N_TILE <= 32 && !I8 ? kTileM * N_TILE * 2 : 0;
+    static constexpr int SCALE_OFFSET = RES_OFFSET + RES_BYTES;
+    static constexpr int SMEM_BYTES = SCALE_OFFSET + (I8 ? (kTileM + N_TILE) * 4 : 0);
     static constexpr int SMEM_ALLOC = SMEM_BYTES + 1024;  // slack to align the base to 1024 B
     // CTAs that fit on one SM (228 KB, 1 KB reserved per CTA), at most 4.
     static constexpr int CTAS_PER_SM = 233472 / (SMEM_ALLOC + 1024) < 4 ? 233472 / (SMEM_ALLOC + 1024) : 4;
@@ -137,11 +148,13 @@ struct ClusterCfg : Cfg<N_TILE, STAGES, 1, FP8> {
 // FP8: the fp8 operand formats and kind::f8f6f4 MMAs; without EPI the
 // output is alpha * acc rounded to fp16, row-major (the dequantisation
 // scale alone).
-template <int N_TILE, int STAGES, bool EPI, bool FP8 = false>
-__global__ void __launch_bounds__(kThreads, ClusterCfg<N_TILE, STAGES, FP8>::CTAS_PER_SM)
+// I8 (with FP8 and EPI): int8 operands, s32 sums, row and column scales.
+template <int N_TILE, int STAGES, bool EPI, bool FP8 = false, bool I8 = false>
+__global__ void __launch_bounds__(kThreads, ClusterCfg<N_TILE, STAGES, FP8, I8>::CTAS_PER_SM)
 spmm24_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                       const __grid_constant__ CUtensorMap tmE, const ClusterParams p) {
-    using C_ = ClusterCfg<N_TILE, STAGES, FP8>;
+    static_assert(!I8 || (FP8 && EPI), "the int8 form is the fp8 one with s32 sums and the general epilogue");
+    using C_ = ClusterCfg<N_TILE, STAGES, FP8, I8>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + C_::BAR_OFFSET);
@@ -259,6 +272,21 @@ spmm24_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
             }
         }
     }
+    // int8: the owner rows' and the tile columns' scales likewise.
+    float* wscale_s = reinterpret_cast<float*>(smem + C_::SCALE_OFFSET);
+    float* xscale_s = wscale_s + kTileM;
+    if constexpr (I8) {
+        if (warp >= 2) {
+            ptx::grid_dep_wait();
+            const int t = threadIdx.x - 64;
+            const int gm = m_tile * kTileM + my_start + t;
+            if (t < my_end - my_start) wscale_s[t] = !p.w_scale ? 1.f : gm < p.M ? p.w_scale[gm] : 0.f;
+            for (int c = t; c < N_TILE; c += kEpiThreads) {
+                const int gn = n_tile * N_TILE + c;
+                xscale_s[c] = !p.x_scale ? 1.f : gn < p.N ? p.x_scale[gn] : 0.f;
+            }
+        }
+    }
 
     if (warp == 1) {
         // ------------------------------------------------------ MMA issuer
@@ -277,9 +305,9 @@ spmm24_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
             if (2 * (st_begin + it) + 1 >= p.groups) patch_tail_metadata<C_>(smem + s * C_::STAGE_BYTES, lane);
             if (lane == 0) {
                 if constexpr (FP8)
-                    mma_stage_fp8<C_, N_TILE>(smem_base + s * C_::STAGE_BYTES,
-                                              tmem_base + C_::META_COL + C_::META_STRIDE * s, tmem_base, accumulate,
-                                              p.mma_fmt);
+                    mma_stage_fp8<C_, N_TILE, I8>(smem_base + s * C_::STAGE_BYTES,
+                                                  tmem_base + C_::META_COL + C_::META_STRIDE * s, tmem_base, accumulate,
+                                                  p.mma_fmt);
                 else
                     mma_stage<C_, N_TILE>(smem_base + s * C_::STAGE_BYTES, tmem_base + C_::META_COL + 4 * s,
                                           tmem_base, accumulate, (EPI && p.epi.bf16) ? kIdescBf16 : 0u);
@@ -359,14 +387,27 @@ spmm24_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
             const int lr = packed ? w % nrows : w / CHUNKS;
             const int ch = packed ? w / nrows : w % CHUNKS;
             float acc[8];
+            if constexpr (I8) {  // the partial tiles hold s32 words
+                int sum[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+                for (int src = 0; src < S; ++src) {
+                    const float* r = red + ((size_t)src * rows_per + lr) * C_::RED_PITCH + ch * 8;
+                    const int4 x0 = *reinterpret_cast<const int4*>(r);
+                    const int4 x1 = *reinterpret_cast<const int4*>(r + 4);
+                    sum[0] += x0.x; sum[1] += x0.y; sum[2] += x0.z; sum[3] += x0.w;
+                    sum[4] += x1.x; sum[5] += x1.y; sum[6] += x1.z; sum[7] += x1.w;
+                }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) acc[e] = 0.f;
-            for (int src = 0; src < S; ++src) {
-                const float* r = red + ((size_t)src * rows_per + lr) * C_::RED_PITCH + ch * 8;
-                const float4 x0 = *reinterpret_cast<const float4*>(r);
-                const float4 x1 = *reinterpret_cast<const float4*>(r + 4);
-                acc[0] += x0.x; acc[1] += x0.y; acc[2] += x0.z; acc[3] += x0.w;
-                acc[4] += x1.x; acc[5] += x1.y; acc[6] += x1.z; acc[7] += x1.w;
+                for (int e = 0; e < 8; ++e) acc[e] = int8_value(sum[e], wscale_s[lr], xscale_s[ch * 8 + e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+                for (int src = 0; src < S; ++src) {
+                    const float* r = red + ((size_t)src * rows_per + lr) * C_::RED_PITCH + ch * 8;
+                    const float4 x0 = *reinterpret_cast<const float4*>(r);
+                    const float4 x1 = *reinterpret_cast<const float4*>(r + 4);
+                    acc[0] += x0.x; acc[1] += x0.y; acc[2] += x0.z; acc[3] += x0.w;
+                    acc[4] += x1.x; acc[5] += x1.y; acc[6] += x1.z; acc[7] += x1.w;
+                }
             }
             const int gm = m0 + my_start + lr;
             const int gn = n0 + ch * 8;
@@ -405,7 +446,8 @@ spmm24_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
 // metadata groups.
 // HALF_N_: 128 (256 x 256 tiles), or 64 (256 x 128 tiles, for shapes with
 // less than half a wave of the wide ones).
-template <int STAGES, bool FP8 = false, int HALF_N_ = 128>
+// I8: shared memory for the tile columns' scales as well.
+template <int STAGES, bool FP8 = false, int HALF_N_ = 128, bool I8 = false>
 struct PairCfg {
     static_assert(HALF_N_ == 64 || HALF_N_ == 128, "pair tiles are 256 or 128 columns wide");
     static constexpr bool kFp8 = FP8;
@@ -419,8 +461,9 @@ struct PairCfg {
     static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
     static constexpr int BAR_OFFSET = RING_BYTES;
     static constexpr int NUM_BARS = 2 * STAGES + 3;  // full, empty, acc_full, recv (pair 0), free (pair 1)
-    static constexpr int HOLDER_OFFSET = BAR_OFFSET + NUM_BARS * 8;
-    static constexpr int SMEM_BYTES = HOLDER_OFFSET + 16;
+    static constexpr int HOLDER_OFFSET = (BAR_OFFSET + NUM_BARS * 8 + 15) / 16 * 16;
+    static constexpr int SCALE_OFFSET = HOLDER_OFFSET + 16;
+    static constexpr int SMEM_BYTES = SCALE_OFFSET + (I8 ? TILE_N * 4 : 0);
     static constexpr int SMEM_ALLOC = SMEM_BYTES + 1024;
     static constexpr int META_COL = TILE_N;  // accumulator: TILE_N fp32 columns
     static constexpr int META_STRIDE = FP8 ? 8 : 4;
@@ -482,13 +525,15 @@ __host__ __device__ constexpr uint32_t pair_idesc_fp8() {
 // EPI: the general epilogue, as for spmm24_cluster_kernel.  KSPLIT: a
 // cluster of two pairs, each taking half of the 128-K stages (p.split == 2;
 // not with a residual, whose staging the partner partial would overlap).
-// FP8: fp8 operand formats and kind::f8f6f4 MMAs (always with EPI).
-template <int STAGES, bool EPI, bool KSPLIT, bool FP8 = false, int HALF_N = 128>
+// FP8: fp8 operand formats and kind::f8f6f4 MMAs (always with EPI).  I8: int8
+// operands in the fp8 layouts, kind::i8 MMAs, row and column scales.
+template <int STAGES, bool EPI, bool KSPLIT, bool FP8 = false, int HALF_N = 128, bool I8 = false>
 __global__ void __launch_bounds__(kPairThreads, 1)
 spmm24_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ CUtensorMap tmE, const PairParams p) {
     static_assert(EPI || !FP8, "the fp8 kernel always runs the general epilogue");
-    using C_ = PairCfg<STAGES, FP8, HALF_N>;
+    static_assert(FP8 || !I8, "the int8 form is the fp8 one with s32 sums");
+    using C_ = PairCfg<STAGES, FP8, HALF_N, I8>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + C_::BAR_OFFSET);  // used in the leader only
@@ -599,8 +644,9 @@ spmm24_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         __syncwarp();
     } else if (warp == 1 && leader) {
         // ---------------------------------- MMA issuer (leader CTA only)
-        const uint32_t idesc = FP8 ? pair_idesc_fp8<C_::TILE_N>() | p.mma_fmt
-                                   : pair_idesc<C_::TILE_N>() | ((EPI && p.epi.bf16) ? kIdescBf16 : 0u);
+        const uint32_t idesc = I8    ? (pair_idesc_fp8<C_::TILE_N>() & ~kIdescF32) | kIdescInt8
+                               : FP8 ? pair_idesc_fp8<C_::TILE_N>() | p.mma_fmt
+                                     : pair_idesc<C_::TILE_N>() | ((EPI && p.epi.bf16) ? kIdescBf16 : 0u);
         const uint32_t smem_base = ptx::smem_u32(smem);
         uint32_t accumulate = 0;
         for (int it = 0; it < st_count; ++it) {
@@ -625,7 +671,10 @@ spmm24_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
                     for (int j = 0; j < 4; ++j) {
                         const uint64_t adesc = smem_desc(st + j * 4096, 2048, 128);
                         const uint64_t bdesc = smem_desc_sw128(stB + (j >> 1) * (C_::B_BYTES / 2) + (j & 1) * 64);
-                        ptx::mma_sp_f8_pair(tmem_base, adesc, bdesc, meta_col + 2 * j, idesc, accumulate);
+                        if constexpr (I8)
+                            ptx::mma_sp_i8_pair(tmem_base, adesc, bdesc, meta_col + 2 * j, idesc, accumulate);
+                        else
+                            ptx::mma_sp_f8_pair(tmem_base, adesc, bdesc, meta_col + 2 * j, idesc, accumulate);
                         accumulate = 1;
                     }
                 } else {
@@ -646,9 +695,20 @@ spmm24_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         if (lane == 0) ptx::tc_commit_pair_mc(acc_full, pair_mask);
         __syncwarp();
     }
+    float* xscale_s = reinterpret_cast<float*>(smem + C_::SCALE_OFFSET);
+    if constexpr (I8) {
+        if (warp >= 4) {  // idle until the accumulator is ready: bring the column scales in
+            ptx::grid_dep_wait();
+            for (int c = threadIdx.x - 128; c < C_::TILE_N; c += kPairThreads - 128) {
+                const int gn = n_tile * C_::TILE_N + c;
+                xscale_s[c] = !p.x_scale ? 1.f : gn < p.N ? p.x_scale[gn] : 0.f;
+            }
+        }
+    }
     {
         // ---------------------------------- epilogue (every warp, both CTAs)
         if (!ptx::mbar_wait_bounded(acc_full, 0, kWaitLimitNs)) atomicOr(&g_spmm24_status, kStatusEpilogueTimeout);
+        if constexpr (I8) ptx::named_barrier(kBarEpi, kPairThreads);  // the scales are in shared memory
         if (threadIdx.x == 64) SPMM24_STAMP(4);
         ptx::tc_fence_after();
         __syncwarp();
@@ -699,6 +759,13 @@ spmm24_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const float4 x = pp[q];
+                    if constexpr (I8) {
+                        v[4 * q] += __float_as_uint(x.x);
+                        v[4 * q + 1] += __float_as_uint(x.y);
+                        v[4 * q + 2] += __float_as_uint(x.z);
+                        v[4 * q + 3] += __float_as_uint(x.w);
+                        continue;
+                    }
                     v[4 * q] = __float_as_uint(__uint_as_float(v[4 * q]) + x.x);
                     v[4 * q + 1] = __float_as_uint(__uint_as_float(v[4 * q + 1]) + x.y);
                     v[4 * q + 2] = __float_as_uint(__uint_as_float(v[4 * q + 2]) + x.z);
@@ -781,7 +848,7 @@ spmm24_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             const int strips = (p.N + 7) / 8;
             constexpr int CH = C_::TILE_N / 8;  // 8-column chunks per row
             constexpr int ITEMS = kTileM * CH;   // (row, chunk) items of this CTA
-            if (p.epi.bias || has_res) ptx::grid_dep_wait();  // they may be written by the previous grid
+            if (I8 || p.epi.bias || has_res) ptx::grid_dep_wait();  // they may be written by the previous grid
             uint4* rst = reinterpret_cast<uint4*>(smem + C_::RES_OFFSET);  // residual tile [row][chunk]
             if (has_res && vec_res) {
                 // packed C: consecutive threads take consecutive rows of a
@@ -798,6 +865,7 @@ spmm24_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             float* fst = reinterpret_cast<float*>(smem);
             uint16_t* hst = reinterpret_cast<uint16_t*>(smem);
             const int gm = gm0 + row;
+            const float wsc = I8 && p.w_scale && gm < p.M ? p.w_scale[gm] : 1.f;
             if (has_res) {
 #pragma unroll 1
                 for (int c = c_begin; c < c_end; ++c) {
@@ -807,7 +875,8 @@ spmm24_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
                     add_partial(v, c);
                     float f[16];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) f[e] = __uint_as_float(v[e]);
+                    for (int e = 0; e < 16; ++e)
+                        f[e] = I8 ? int8_value((int)v[e], wsc, xscale_s[c * 16 + e]) : __uint_as_float(v[e]);
                     if (gm < p.M) epilogue_pre<16>(f, p.epi, gm);
                     float4* dst = reinterpret_cast<float4*>(fst + (size_t)row * C_::F_PITCH + c * 16);
 #pragma unroll
@@ -823,7 +892,8 @@ spmm24_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
                     add_partial(v, c);
                     float f[16];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) f[e] = __uint_as_float(v[e]);
+                    for (int e = 0; e < 16; ++e)
+                        f[e] = I8 ? int8_value((int)v[e], wsc, xscale_s[c * 16 + e]) : __uint_as_float(v[e]);
                     if (gm < p.M) epilogue_pre<16>(f, p.epi, gm);
                     const int gn = gn0 + c * 16;
                     uint32_t h[8];
@@ -942,11 +1012,12 @@ spmm24_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
 // one per stage (the copy into a slot is issued after the MMAs that read
 // it two stages earlier, and tcgen05 operations of one thread execute in
 // issue order), which leaves room for the two 240-column accumulators;
-// always EPI.
-template <int STAGES, bool FP8 = false>
+// always EPI.  I8: 512 x 224 tiles (kind::i8 with M = 256 takes N in steps of
+// 32), row and column scales.
+template <int STAGES, bool FP8 = false, bool I8 = false>
 struct Pair2Cfg {
     static constexpr bool kFp8 = FP8;
-    static constexpr int HALF_N = 120;                   // columns of B / C per CTA
+    static constexpr int HALF_N = I8 ? 112 : 120;        // columns of B / C per CTA
     static constexpr int TILE_N = 2 * HALF_N;            // columns per pair
     static constexpr int TILE_M = 4 * kTileM;            // rows per pair
     static constexpr int A_HALF = 8 * 8 * 256;           // 128 rows x 128 logical K (fp8: 256)
@@ -960,8 +1031,9 @@ struct Pair2Cfg {
     static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
     static constexpr int BAR_OFFSET = RING_BYTES;
     static constexpr int NUM_BARS = 2 * STAGES + 1;  // full, empty, acc_full
-    static constexpr int HOLDER_OFFSET = BAR_OFFSET + NUM_BARS * 8;
-    static constexpr int SMEM_BYTES = HOLDER_OFFSET + 16;
+    static constexpr int HOLDER_OFFSET = (BAR_OFFSET + NUM_BARS * 8 + 15) / 16 * 16;
+    static constexpr int SCALE_OFFSET = HOLDER_OFFSET + 16;
+    static constexpr int SMEM_BYTES = SCALE_OFFSET + (I8 ? TILE_N * 4 : 0);
     static constexpr int SMEM_ALLOC = SMEM_BYTES + 1024;
     static constexpr int ACC1_COL = 256;                  // second accumulator
     static constexpr int META0_COL = TILE_N;              // metadata rings after each accumulator
@@ -976,12 +1048,13 @@ struct Pair2Cfg {
                   "fp8 B halves must start on 1024-byte boundaries (128-byte swizzle atoms)");
 };
 
-template <int STAGES, bool EPI, bool FP8 = false>
+template <int STAGES, bool EPI, bool FP8 = false, bool I8 = false>
 __global__ void __launch_bounds__(kPairThreads, 1)
 spmm24_pair2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmE, const PairParams p) {
     static_assert(EPI || !FP8, "the fp8 form always runs the epilogue (alpha)");
-    using C_ = Pair2Cfg<STAGES, FP8>;
+    static_assert(FP8 || !I8, "the int8 form is the fp8 one with s32 sums");
+    using C_ = Pair2Cfg<STAGES, FP8, I8>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + C_::BAR_OFFSET);  // used in the leader only
@@ -1095,8 +1168,9 @@ spmm24_pair2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         __syncwarp();
     } else if (warp == 1 && leader) {
         // ---------------------------------- MMA issuer (leader CTA only)
-        const uint32_t idesc = FP8 ? pair_idesc_fp8<C_::TILE_N>() | p.mma_fmt
-                                   : pair_idesc<C_::TILE_N>() | ((EPI && p.epi.bf16) ? kIdescBf16 : 0u);
+        const uint32_t idesc = I8    ? (pair_idesc_fp8<C_::TILE_N>() & ~kIdescF32) | kIdescInt8
+                               : FP8 ? pair_idesc_fp8<C_::TILE_N>() | p.mma_fmt
+                                     : pair_idesc<C_::TILE_N>() | ((EPI && p.epi.bf16) ? kIdescBf16 : 0u);
         const uint32_t smem_base = ptx::smem_u32(smem);
         uint32_t accumulate = 0;
         for (int it = 0; it < st_count; ++it) {
@@ -1124,10 +1198,15 @@ spmm24_pair2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const uint64_t bdesc = smem_desc_sw128(stB + (j >> 1) * (C_::B_BYTES / 2) + (j & 1) * 64);
-                        ptx::mma_sp_f8_pair(tmem_base, smem_desc(st + j * 4096, 2048, 128), bdesc, meta0 + 2 * j, idesc,
-                                            accumulate);
-                        ptx::mma_sp_f8_pair(tmem_base + C_::ACC1_COL, smem_desc(st + C_::A_HALF + j * 4096, 2048, 128),
-                                            bdesc, meta1 + 2 * j, idesc, accumulate);
+                        const uint64_t a0 = smem_desc(st + j * 4096, 2048, 128);
+                        const uint64_t a1 = smem_desc(st + C_::A_HALF + j * 4096, 2048, 128);
+                        if constexpr (I8) {
+                            ptx::mma_sp_i8_pair(tmem_base, a0, bdesc, meta0 + 2 * j, idesc, accumulate);
+                            ptx::mma_sp_i8_pair(tmem_base + C_::ACC1_COL, a1, bdesc, meta1 + 2 * j, idesc, accumulate);
+                        } else {
+                            ptx::mma_sp_f8_pair(tmem_base, a0, bdesc, meta0 + 2 * j, idesc, accumulate);
+                            ptx::mma_sp_f8_pair(tmem_base + C_::ACC1_COL, a1, bdesc, meta1 + 2 * j, idesc, accumulate);
+                        }
                         accumulate = 1;
                     }
                 } else {
@@ -1152,6 +1231,16 @@ spmm24_pair2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         if (lane == 0) ptx::tc_commit_pair_mc(acc_full, (uint16_t)0x3);
         __syncwarp();
     }
+    float* xscale_s = reinterpret_cast<float*>(smem + C_::SCALE_OFFSET);
+    if constexpr (I8) {
+        if (warp >= 4) {  // idle until the accumulators are ready: bring the column scales in
+            ptx::grid_dep_wait();
+            for (int c = threadIdx.x - 128; c < C_::TILE_N; c += kPairThreads - 128) {
+                const int gn = n_tile * C_::TILE_N + c;
+                xscale_s[c] = !p.x_scale ? 1.f : gn < p.N ? p.x_scale[gn] : 0.f;
+            }
+        }
+    }
     {
         // ------------------------------- epilogue (every warp, both CTAs)
         // TMEM -> (EPI: alpha, bias, activation) -> 16-bit -> staged rows
@@ -1162,12 +1251,18 @@ spmm24_pair2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         __syncwarp();
         const int quad = warp & 3;
         const int row = quad * 32 + lane;
-        constexpr int NCH16 = C_::TILE_N / 16;          // chunks of 16 columns per row (15; fp8 14)
+        constexpr int NCH16 = C_::TILE_N / 16;          // chunks of 16 columns per row (15; int8 14)
         const int c_begin = (warp >> 2) ? (NCH16 + 1) / 2 : 0;  // warps 0-3 take the first half
         const int c_end = (warp >> 2) ? NCH16 : (NCH16 + 1) / 2;
         __half* cst = reinterpret_cast<__half*>(smem);
+        if constexpr (I8) {
+            ptx::named_barrier(kBarEpi, kPairThreads);  // the scales are in shared memory
+            ptx::grid_dep_wait();
+        }
 #pragma unroll 1
         for (int h = 0; h < 2; ++h) {
+            const int gmh = m_tile * C_::TILE_M + h * 2 * kTileM + (int)rank * kTileM + row;
+            const float wsc = I8 && p.w_scale && gmh < p.M ? p.w_scale[gmh] : 1.f;
 #pragma unroll 1
             for (int c = c_begin; c < c_end; ++c) {
                 uint32_t v[16];
@@ -1179,9 +1274,9 @@ spmm24_pair2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                 if constexpr (EPI) {
                     float y[16];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) y[e] = __uint_as_float(v[e]);
-                    const int gm = m_tile * C_::TILE_M + h * 2 * kTileM + (int)rank * kTileM + row;
-                    if (gm < p.M) epilogue_pre<16>(y, p.epi, gm);
+                    for (int e = 0; e < 16; ++e)
+                        y[e] = I8 ? int8_value((int)v[e], wsc, xscale_s[c * 16 + e]) : __uint_as_float(v[e]);
+                    if (gmh < p.M) epilogue_pre<16>(y, p.epi, gmh);
                     uint32_t w[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) w[e] = pack2(y[2 * e], y[2 * e + 1], p.epi.bf16);
@@ -1199,8 +1294,8 @@ spmm24_pair2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         ptx::tc_fence_before();
         ptx::named_barrier(kBarEpi, kPairThreads);
         ptx::grid_dep_wait();  // C may be in use by the previous grid
-        constexpr int LPR = C_::TILE_N / 8;      // threads per row (30; fp8 28)
-        constexpr int RPP = kPairThreads / LPR;  // rows per pass (8; fp8 9)
+        constexpr int LPR = C_::TILE_N / 8;      // threads per row (30; int8 28)
+        constexpr int RPP = kPairThreads / LPR;  // rows per pass (8; int8 9)
         const int etid = threadIdx.x;
         bool packed_out = false;
         if constexpr (EPI) packed_out = p.epi.packed != 0;

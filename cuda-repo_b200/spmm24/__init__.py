@@ -118,6 +118,21 @@ _lib.spmm24_launch_fp8.argtypes = [_vp, _vp, _vp, _vp, _vp, ctypes.c_int, ctypes
 _lib.spmm24_launch_fp8.restype = ctypes.c_int
 _lib.spmm24_pack_a_fp8_device.argtypes = [_vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp, _vp]
 _lib.spmm24_pack_a_fp8_device.restype = ctypes.c_int
+_i8p = ctypes.POINTER(ctypes.c_int8)
+_lib.spmm24_quantize_int8.argtypes = [_vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_longlong, ctypes.c_int,
+                                      ctypes.c_uint, _vp, _vp]
+_lib.spmm24_quantize_int8.restype = ctypes.c_int
+_lib.spmm24_prune_2of4_int8.argtypes = [_i8p, ctypes.c_int, ctypes.c_int]
+_lib.spmm24_prune_2of4_int8.restype = ctypes.c_int
+_lib.spmm24_compress_a_int8.argtypes = [_i8p, ctypes.c_int, ctypes.c_int, _u8p, _u8p]
+_lib.spmm24_compress_a_int8.restype = ctypes.c_int
+_lib.spmm24_pack_a_int8_device.argtypes = [_vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp, _vp]
+_lib.spmm24_pack_a_int8_device.restype = ctypes.c_int
+_lib.spmm24_launch_int8.argtypes = [_vp, _vp, _vp, _vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp,
+                                    ctypes.c_int, ctypes.c_uint, ctypes.c_void_p]
+_lib.spmm24_launch_int8.restype = ctypes.c_int
+_lib.spmm24_select_config_int8.argtypes = [ctypes.c_int] * 4 + [ctypes.POINTER(SpmmConfig)]
+_lib.spmm24_select_config_int8.restype = ctypes.c_int
 _lib.spmm24_workspace_bytes.argtypes = [ctypes.c_int] * 4
 _lib.spmm24_workspace_bytes.restype = ctypes.c_size_t
 _lib.spmm24_select_config.argtypes = [ctypes.c_int] * 4 + [ctypes.POINTER(SpmmConfig)]
@@ -210,6 +225,37 @@ def launch_fp8(stream, values, b_nk, metadata, c, M: int, N: int, K: int, split_
     epi = Epilogue(_ptr(bias), _ptr(residual), float(alpha), int(activation), int(out_layout))
     return _lib.spmm24_launch_fp8(_stream_handle(stream), _ptr(values), _ptr(b_nk), _ptr(metadata), _ptr(c), M, N, K,
                                   split_k, flags, ctypes.addressof(epi))
+
+
+def launch_int8(stream, values, b_nk, metadata, c, M: int, N: int, K: int, w_scale=None, x_scale=None,
+                split_k: int = 0, flags: int = 0, bias=None, residual=None, alpha: float = 1.0,
+                activation: int = ACT_NONE, out_layout: int = OUT_ROW_MAJOR) -> int:
+    """spmm24_launch_int8: C = act(alpha * (w_scale[m] x_scale[n] A_sparse B) +
+    bias) + residual with int8 A (values + metadata in the 8-bit formats) and B
+    as N x K int8; w_scale (M floats) and x_scale (N floats) may be None (1).
+    Returns the cudaError_t code."""
+    epi = Epilogue(_ptr(bias), _ptr(residual), float(alpha), int(activation), int(out_layout))
+    return _lib.spmm24_launch_int8(_stream_handle(stream), _ptr(values), _ptr(b_nk), _ptr(metadata), _ptr(c), M, N, K,
+                                   _ptr(w_scale), _ptr(x_scale), split_k, flags, ctypes.addressof(epi))
+
+
+def quantize_int8(x, rows: int, cols: int, q=None, scale=None, bf16: bool = False, packed: bool = False, ld: int = 0,
+                  stream=None):
+    """spmm24_quantize_int8: rows of 16-bit x (row-major with row stride ld, or
+    packed strips) -> (q: rows x cols int8, scale: rows floats)."""
+    import torch
+
+    if q is None:
+        q = torch.empty((rows, cols), dtype=torch.int8, device=x.device)
+    if scale is None:
+        scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    if stream is None:
+        stream = torch.cuda.current_stream(x.device)
+    rc = _lib.spmm24_quantize_int8(_stream_handle(stream), _ptr(x), rows, cols, ld,
+                                   OUT_PACKED_B if packed else OUT_ROW_MAJOR, BF16 if bf16 else 0, _ptr(q), _ptr(scale))
+    if rc != CUDA_SUCCESS:
+        raise SpmmError(rc, "spmm24_quantize_int8")
+    return q, scale
 
 
 class Problem(ctypes.Structure):
@@ -379,6 +425,14 @@ def select_config_fp8(M: int, N: int, K: int, split_k: int = 0) -> dict:
     cfg = SpmmConfig()
     if _lib.spmm24_select_config_fp8(M, N, K, split_k, ctypes.byref(cfg)) != 0:
         raise ValueError("unsupported shape (K % 128)")
+    return {n: getattr(cfg, n) for n, _ in SpmmConfig._fields_}
+
+
+def select_config_int8(M: int, N: int, K: int, split_k: int = 0) -> dict:
+    """spmm24_select_config_int8: the configuration spmm24_launch_int8 uses."""
+    cfg = SpmmConfig()
+    if _lib.spmm24_select_config_int8(M, N, K, split_k, ctypes.byref(cfg)) != 0:
+        raise ValueError("unsupported shape (K % 128, K < 262144)")
     return {n: getattr(cfg, n) for n, _ in SpmmConfig._fields_}
 
 
@@ -631,6 +685,52 @@ def pack_a_fp8_device(dense, M: int, K: int, prune: int = 0, values=None, meta=N
                                        _ptr(bad_blocks))
     if rc != CUDA_SUCCESS:
         raise SpmmError(rc, "spmm24_pack_a_fp8_device")
+    return values, meta
+
+
+def _i8(a: np.ndarray) -> np.ndarray:
+    a = np.ascontiguousarray(a)
+    if a.dtype != np.int8:
+        raise TypeError("expected int8 data")
+    return a
+
+
+def prune_2of4_int8(dense_a: np.ndarray, M: int, K: int) -> np.ndarray:
+    """Magnitude 2:4 pruning along K of int8 values (returns a pruned copy)."""
+    a = _i8(dense_a).reshape(-1).copy()
+    if _lib.spmm24_prune_2of4_int8(a.ctypes.data_as(_i8p), M, K) != 0:
+        raise ValueError("prune_2of4_int8: K % 4 must be 0")
+    return a
+
+
+def compress_a_int8(dense_a: np.ndarray, M: int, K: int):
+    """(values, metadata) of a 2:4-sparse int8 matrix in the 8-bit SpMM's formats."""
+    d = _i8(dense_a).reshape(-1)
+    vals = np.empty(M * K // 2, dtype=np.uint8)
+    meta = np.empty(M * K // 8, dtype=np.uint8)
+    n = _lib.spmm24_compress_a_int8(d.ctypes.data_as(_i8p), M, K, vals.ctypes.data_as(_u8p), meta.ctypes.data_as(_u8p))
+    if n == -2:
+        raise ValueError("matrix is not 2:4 sparse along K (a group of four has fewer than two zeros)")
+    if n < 0:
+        raise ValueError("compress_a_int8: M % 16 and K % 128 must be 0")
+    return vals, meta
+
+
+def pack_a_int8_device(dense, M: int, K: int, prune: bool = False, values=None, meta=None, bad_blocks=None,
+                       stream=None):
+    """spmm24_pack_a_int8_device on int8 device tensors; returns (values, meta)."""
+    import torch
+
+    if values is None:
+        values = torch.empty(M * K // 2, dtype=torch.uint8, device=dense.device)
+    if meta is None:
+        meta = torch.empty(M * K // 8, dtype=torch.uint8, device=dense.device)
+    if stream is None:
+        stream = torch.cuda.current_stream(dense.device)
+    rc = _lib.spmm24_pack_a_int8_device(_stream_handle(stream), _ptr(dense), M, K, int(prune), _ptr(values), _ptr(meta),
+                                        _ptr(bad_blocks))
+    if rc != CUDA_SUCCESS:
+        raise SpmmError(rc, "spmm24_pack_a_int8_device")
     return values, meta
 
 

@@ -372,6 +372,51 @@ cudaError_t spmm24_pack_a_fp8_device(cudaStream_t stream, const void* dense_a, i
 cudaError_t spmm24_launch_fp8(cudaStream_t stream, const void* values, const void* b_nk, const void* metadata, void* c,
                               int M, int N, int K, int split_k, unsigned flags, const spmm24_epilogue* epilogue);
 
+/* --------------------------------------------------------------- int8
+ * int8 extension (no counterpart in the reference): A and B hold signed
+ * 8-bit integers, the tensor cores run tcgen05.mma.sp kind::i8 with exact
+ * 32-bit sums, and each output row (channel) and column (token) has a scale:
+ *     acc = sum_k A[m, k] B[n, k]                        (exact)
+ *     C[m, n] = act(alpha * (acc * w_scale[m] * x_scale[n]) + bias[m]) + residual[m, n]
+ * Values, metadata and B have the fp8 extension's layouts (K % 128 == 0,
+ * M % 16 == 0, K < 262144), bytes being int8; a weight of -128 is allowed, and
+ * only the byte 0 is a zero.  The sum being exact, every split_k gives the
+ * same bits.  C, bias and residual are fp16 (bf16 with SPMM24_BF16). */
+
+/* 16-bit rows -> int8 rows and one scale for each row: activations (a row =
+ * a token) or weights (a row = an output channel).
+ *     scale[r] = max_k |x[r, k]| / 127,  q[r, k] = rint(127 x[r, k] / max)
+ * exactly, ties to even; values lie in -127 .. 127; a row of zeros has scale
+ * 0; a row that holds an infinity (NaN) has an infinite (NaN) scale and zero
+ * values, so its products are NaN.  scale is the nearest fp32 value.
+ *   layout  SPMM24_OUT_ROW_MAJOR: x[r, k] at r * ld + k (ld 0: cols), any
+ *           cols and alignment (16-byte aligned x, 8-byte aligned q, and cols
+ *           and ld multiples of 8 are the fast case); SPMM24_OUT_PACKED_B: the
+ *           strips that a launch with that output layout writes (rows = its N,
+ *           cols = its M), x 16-byte and q 8-byte aligned, cols % 8 == 0, ld 0
+ *   flags   SPMM24_BF16 (x holds bf16), SPMM24_NO_PDL
+ * q: rows x cols int8, row-major (the b_nk of spmm24_launch_int8); scale:
+ * rows floats.  Asynchronous on `stream`. */
+cudaError_t spmm24_quantize_int8(cudaStream_t stream, const void* x, int rows, int cols, long long ld, int layout,
+                                 unsigned flags, void* q, float* scale);
+/* Magnitude 2:4 prune of a row-major M x K int8 matrix in place (ties prefer
+ * the lower index).  Returns 0 or -1. */
+int spmm24_prune_2of4_int8(int8_t* dense_a, int M, int K);
+/* spmm24_compress_a_fp8 for int8 values: same layouts and return codes. */
+int spmm24_compress_a_int8(const int8_t* dense_a, int M, int K, uint8_t* values_out, uint8_t* meta_out);
+/* spmm24_pack_a_fp8_device for int8 values: prune 0 = none, 1 = by magnitude;
+ * bit-exact with the host functions. */
+cudaError_t spmm24_pack_a_int8_device(cudaStream_t stream, const void* dense_a, int M, int K, int prune,
+                                      void* values_out, void* meta_out, int* bad_blocks);
+/* The int8 product above.  w_scale: M floats, x_scale: N floats, either may
+ * be NULL (1).  split_k, flags (SPMM24_STATIC_WEIGHTS, SPMM24_NO_PDL,
+ * SPMM24_BF16) and epilogue as for spmm24_launch_fused; SPMM24_STATIC_WEIGHTS
+ * covers values and metadata, not the scales.  values, b_nk and metadata
+ * 16-byte aligned.  Asynchronous on `stream`. */
+cudaError_t spmm24_launch_int8(cudaStream_t stream, const void* values, const void* b_nk, const void* metadata, void* c,
+                               int M, int N, int K, const float* w_scale, const float* x_scale, int split_k,
+                               unsigned flags, const spmm24_epilogue* epilogue);
+
 /* Packed-weight files (no counterpart in the reference): a 64-byte header
  * (magic "SPMM24W", version 1, dtype 0 = fp16 / 1 = bf16 / 2 = fp8 E4M3 /
  * 3 = fp8 E5M2, M, K, payload sizes, FNV-1a-64 checksum of the payload),
@@ -453,6 +498,8 @@ int spmm24_group_schedule(const int* M, const int* K, int count, int fp8, int sm
  * K of fp8 operands; K % 128 == 0), for an epilogue without a residual or a
  * packed output. */
 int spmm24_select_config_fp8(int M, int N, int K, int split_k, spmm24_config* out);
+/* The same for spmm24_launch_int8. */
+int spmm24_select_config_int8(int M, int N, int K, int split_k, spmm24_config* out);
 
 /* Row range of shard `index` of `parts` when an M x K layer is split along
  * M across devices (no reduction needed: each shard is a contiguous slice
