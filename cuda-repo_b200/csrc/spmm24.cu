@@ -26,6 +26,7 @@
 #include "spmm24_host.h"
 #include "spmm24_kernel.cuh"
 #include "spmm24_grouped.cuh"
+#include "spmm24_moe.cuh"
 
 namespace spmm24 {
 
@@ -1181,6 +1182,182 @@ cudaError_t launch_grouped_impl(cudaStream_t stream, const spmm24_problem* probs
     return launch_group_kernel<false, false, 1>(stream, dev, gc, flags);
 }
 
+// ------------------------------------------------ mixture-of-experts layer
+// The workspace: counters first, at the same place for every layer's sizes
+// (they are zero between launches, whatever layers share the workspace).
+struct MoeLayout {
+    size_t tile_count, logits, xscale, amax, part, xq, h, hq, total;
+    int slots, shares;
+};
+
+int moe_ctas(int sms) { return std::min(sms, kMoeMaxCtas); }
+
+MoeLayout moe_layout(int T, int H, int I, int E, int k, bool i8) {
+    MoeLayout l{};
+    size_t at = 0;
+    auto take = [&at](size_t bytes) {
+        const size_t here = at;
+        at = (at + bytes + 255) / 256 * 256;
+        return here;
+    };
+    const int strips = (T + 7) / 8, n_tile = T <= 16 ? 16 : 32;
+    l.slots = std::min(E, T * k);
+    // enough K shares of a logit to give every warp of the device one, of at
+    // least 256 inputs (one load of a warp)
+    l.shares = std::max(1, std::min({kMoeMaxCtas * kMoeWarps / (E * strips), (H + 255) / 256, 32}));
+    take(256);
+    l.tile_count = take((size_t)(kMoeMaxTiles + kMoeMaxDownTiles) * 4);
+    l.logits = take((size_t)l.shares * T * E * 4);
+    l.xscale = take(kMoeMaxTokens * 4);
+    l.amax = take((size_t)l.slots * kMoeMaxTokens * 4);
+    l.part = take((size_t)kMoeMaxCtas * 2 * kTileM * 2 * n_tile * 4);
+    l.xq = take(i8 ? (size_t)T * H : 0);
+    l.h = take(i8 ? (size_t)l.slots * T * I * 4 : (size_t)l.slots * strips * I * 16);
+    l.hq = take(i8 ? (size_t)l.slots * T * I : 0);
+    l.total = at;
+    return l;
+}
+
+// The sizes of a layer; null if it is supported, else why not.
+const char* moe_sizes(int T, int H, int I, int E, int k, bool i8) {
+    if (T < 1 || T > kMoeMaxTokens) return "moe: tokens must be 1..32";
+    if (E < 1 || E > kMoeMaxExperts) return "moe: experts must be 1..256";
+    if (k < 1 || k > E || k > kMoeMaxTopK) return "moe: top_k must be 1..min(experts, 16)";
+    const int step = i8 ? 128 : 64;
+    if (H < step || I < step || H % step || I % step)
+        return i8 ? "moe int8: hidden and inter must be positive multiples of 128"
+                  : "moe: hidden and inter must be positive multiples of 64";
+    if (H > 131072 || I > 131072) return "moe: hidden and inter must be <= 131072";
+    if ((long long)std::min(E, T * k) * ((I + kTileM - 1) / kTileM) > kMoeMaxTiles)
+        return "moe: min(experts, tokens * top_k) * ceil(inter / 128) must be <= 32768";
+    return nullptr;
+}
+
+template <int N_TILE, bool I8>
+cudaError_t launch_moe_kernel(cudaStream_t stream, int dev, int ctas, const MoeParams& mp) {
+    using MC = MoeCfg<N_TILE, I8>;
+    auto kern = spmm24_moe_kernel<N_TILE, I8>;
+    cudaError_t e = prepare(kern, MC::SMEM_ALLOC, dev, 112 + (N_TILE == 32 ? 1 : 0) + (I8 ? 2 : 0));
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas, 1, 1);
+    cfg.blockDim = dim3((unsigned)kThreads, 1, 1);
+    cfg.dynamicSmemBytes = MC::SMEM_ALLOC;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeCooperative;  // the CTAs wait for one another: all resident, or none
+    attr[0].val.cooperative = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, mp);
+}
+
+cudaError_t launch_moe_impl(cudaStream_t stream, const spmm24_moe_layer* L, unsigned flags) {
+    g_last_error[0] = '\0';
+    if (!L) return invalid("moe: null layer");
+    if (flags & ~(unsigned)(SPMM24_BF16 | SPMM24_MOE_INT8 | SPMM24_STATIC_WEIGHTS | SPMM24_NO_PDL))
+        return invalid("unknown flag");
+    const bool i8 = flags & SPMM24_MOE_INT8;
+    const int T = L->tokens, H = L->hidden, I = L->inter, E = L->experts, k = L->top_k;
+    if (const char* why = moe_sizes(T, H, I, E, k, i8)) return invalid(why);
+    if (!L->x || !L->gate_up || !L->gate_up_meta || !L->down || !L->down_meta || !L->y || !L->workspace)
+        return invalid("moe: null pointer");
+    if (((uintptr_t)L->x | (uintptr_t)L->router | (uintptr_t)L->gate_up | (uintptr_t)L->gate_up_meta |
+         (uintptr_t)L->down | (uintptr_t)L->down_meta) & 15u)
+        return invalid("moe: x, router, weights and metadata must be 16-byte aligned");
+    if (((uintptr_t)L->topk_ids | (uintptr_t)L->topk_weights | (uintptr_t)L->gate_up_scale | (uintptr_t)L->down_scale) & 3u)
+        return invalid("moe: top-k ids and weights and the scales must be 4-byte aligned");
+    if ((uintptr_t)L->y & 1u) return invalid("moe: y must be 2-byte aligned");
+    if (!L->router && (!L->topk_ids || !L->topk_weights))
+        return invalid("moe: without a router, topk_ids and topk_weights are inputs");
+    if (i8 != (L->gate_up_scale && L->down_scale) || (!i8 && (L->gate_up_scale || L->down_scale)))
+        return invalid("moe: int8 experts take both scales, 16-bit experts none");
+    if (L->activation < SPMM24_ACT_NONE || L->activation > SPMM24_ACT_GELU) return invalid("moe: unknown activation");
+    const MoeLayout lay = moe_layout(T, H, I, E, k, i8);
+    if ((uintptr_t)L->workspace & 255u) return invalid("moe: the workspace must be 256-byte aligned");
+    if (L->workspace_bytes < lay.total) return invalid("moe: the workspace is too small (spmm24_moe_workspace_bytes)");
+    MoeParams mp{};
+    cudaError_t e = make_epilogue(L->epilogue, flags, L->y, &mp.epi);
+    if (e != cudaSuccess) return e;
+    int dev = 0;
+    if ((e = cudaGetDevice(&dev)) != cudaSuccess) return e;
+
+    uint8_t* ws = static_cast<uint8_t*>(L->workspace);
+    mp.x = static_cast<const uint16_t*>(L->x);
+    mp.router = static_cast<const uint16_t*>(L->router);
+    mp.ids = L->topk_ids;
+    mp.weights = L->topk_weights;
+    mp.gu_scale = L->gate_up_scale;
+    mp.d_scale = L->down_scale;
+    mp.y = static_cast<uint16_t*>(L->y);
+    mp.T = T;
+    mp.H = H;
+    mp.I = I;
+    mp.E = E;
+    mp.k = k;
+    mp.strips = (T + 7) / 8;
+    mp.act = L->activation;
+    mp.norm = L->norm_topk ? 1 : 0;
+    mp.bf16 = (flags & SPMM24_BF16) ? 1 : 0;
+    mp.max_slots = lay.slots;
+    mp.logit_shares = lay.shares;
+    mp.bar = reinterpret_cast<uint32_t*>(ws);
+    mp.tile_count = reinterpret_cast<uint32_t*>(ws + lay.tile_count);
+    mp.logits = reinterpret_cast<float*>(ws + lay.logits);
+    mp.xscale = reinterpret_cast<float*>(ws + lay.xscale);
+    mp.amax = reinterpret_cast<uint32_t*>(ws + lay.amax);
+    mp.part = reinterpret_cast<float*>(ws + lay.part);
+    mp.xq = reinterpret_cast<int8_t*>(ws + lay.xq);
+    mp.h32 = reinterpret_cast<float*>(ws + lay.h);
+    mp.h16 = reinterpret_cast<uint16_t*>(ws + lay.h);
+    mp.hq = reinterpret_cast<int8_t*>(ws + lay.hq);
+
+    // Weights: all experts' rows stacked (the packed forms of matrices of the
+    // same K follow one another).
+    auto weight_maps = [&](CUtensorMap* ta, CUtensorMap* te, const void* A, const void* M_, size_t rows, int K) {
+        const int Ka = i8 ? K / 2 : K;
+        cuuint64_t adims[3] = {128, (cuuint64_t)(rows / 16), (cuuint64_t)(Ka / 16)};
+        cuuint64_t astr[2] = {(cuuint64_t)16 * Ka, 256};
+        cuuint32_t abox[3] = {128, 8, 8};
+        if (!encode(ta, 3, A, adims, astr, abox)) return false;
+        if (i8) {
+            cuuint64_t edims[3] = {128, (cuuint64_t)(rows / 16), (cuuint64_t)(K / 128)};
+            cuuint64_t estr[2] = {(cuuint64_t)(K / 128) * 256, 256};
+            cuuint32_t ebox[3] = {128, 8, 2};
+            return encode(te, 3, M_, edims, estr, ebox);
+        }
+        cuuint64_t edims[2] = {(cuuint64_t)K, (cuuint64_t)(rows / 16)};
+        cuuint64_t estr[1] = {(cuuint64_t)2 * K};
+        cuuint32_t ebox[2] = {128, 8};
+        return encode(te, 2, M_, edims, estr, ebox);
+    };
+    const int n_tile = T <= 16 ? 16 : 32;
+    // Activations of `slots` experts: strips, or (int8) rows of each slot.
+    auto act_map = [&](CUtensorMap* tb, const void* B, int K, int slots) {
+        if (i8) {
+            cuuint64_t dims[3] = {(cuuint64_t)K, (cuuint64_t)T, (cuuint64_t)slots};
+            cuuint64_t str[2] = {(cuuint64_t)K, (cuuint64_t)K * T};
+            cuuint32_t box[3] = {128, (cuuint32_t)n_tile, 1};
+            return encode(tb, 3, B, dims, str, box, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B);
+        }
+        cuuint64_t dims[4] = {128, (cuuint64_t)(K / 64), 4, (cuuint64_t)slots * mp.strips};
+        cuuint64_t str[3] = {1024, 256, (cuuint64_t)16 * K};
+        cuuint32_t box[4] = {128, 2, 4, (cuuint32_t)mp.strips};
+        return encode(tb, 4, B, dims, str, box);
+    };
+    if (!weight_maps(&mp.tmGU, &mp.tmGUE, L->gate_up, L->gate_up_meta, (size_t)E * 2 * I, H) ||
+        !weight_maps(&mp.tmD, &mp.tmDE, L->down, L->down_meta, (size_t)E * H, I) ||
+        !act_map(&mp.tmX, i8 ? (const void*)mp.xq : L->x, H, 1) ||
+        !act_map(&mp.tmH, i8 ? (const void*)mp.hq : (const void*)mp.h16, I, lay.slots))
+        return invalid("moe: a TMA descriptor could not be encoded");
+    const int ctas = moe_ctas(sm_count(dev));
+    if (i8)
+        return n_tile == 16 ? launch_moe_kernel<16, true>(stream, dev, ctas, mp)
+                            : launch_moe_kernel<32, true>(stream, dev, ctas, mp);
+    return n_tile == 16 ? launch_moe_kernel<16, false>(stream, dev, ctas, mp)
+                        : launch_moe_kernel<32, false>(stream, dev, ctas, mp);
+}
+
 // ------------------------------------------------ allocation-free variant
 // Scratch for spmm24_launch_noalloc, owned by the library as a file-scope
 // device array instead of a cudaMalloc'ed buffer: 256 flag words followed by
@@ -1430,6 +1607,16 @@ extern "C" cudaError_t spmm24_launch_int8(cudaStream_t stream, const void* value
                                           const spmm24_epilogue* epilogue) {
     return spmm24::launch_fp8_impl(stream, values, b_nk, metadata, c, M, N, K, split_k, flags, epilogue, true, w_scale,
                                    x_scale);
+}
+
+extern "C" cudaError_t spmm24_launch_moe(cudaStream_t stream, const spmm24_moe_layer* layer, unsigned flags) {
+    return spmm24::launch_moe_impl(stream, layer, flags);
+}
+
+extern "C" size_t spmm24_moe_workspace_bytes(int tokens, int hidden, int inter, int experts, int top_k, unsigned flags) {
+    const bool i8 = flags & SPMM24_MOE_INT8;
+    if (spmm24::moe_sizes(tokens, hidden, inter, experts, top_k, i8)) return 0;
+    return spmm24::moe_layout(tokens, hidden, inter, experts, top_k, i8).total;
 }
 
 extern "C" cudaError_t spmm24_launch_gather(cudaStream_t stream, const void* compressed_a, const void* b_packed,

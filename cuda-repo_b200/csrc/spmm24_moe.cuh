@@ -1,0 +1,852 @@
+// spmm24_moe.cuh -- a whole mixture-of-experts layer for a few tokens (T <= 32)
+// in one persistent launch, 2:4-sparse experts in fp16, bf16 or int8.
+//
+//   l[t, e] = sum_i router[e, i] x[t, i]              (fp32)
+//   E_t     = the k largest l[t, .], ties to the lower expert
+//   w[t, j] = softmax(l[t, .])[E_t[j]], optionally divided by their sum
+//   h[t, j] = act(Wg_e x_t) * (Wu_e x_t)              e = E_t[j]
+//   y[t]    = sum_j w[t, j] Wd_e h[t, j]
+//
+// int8 experts: x_t is rounded to int8 with its own scale (int8_rows.cuh),
+// every h[t, j] likewise with the scale of its own largest value, products are
+// exact 32-bit sums times the channel's and the row's scale.  16-bit experts:
+// h is rounded once to the operand type, which a 16-bit product needs.
+//
+// Bound by the chosen experts' weights, each read once: 3 I H values of 9/8
+// (16-bit) or 5/8 bytes per expert that some token chose.  So one CTA per SM
+// streams weights through a TMA ring without a stop, as the grouped kernel
+// does, and everything else is arranged around that:
+//
+//   - All T tokens are the columns of every product (an expert's other columns
+//     are not used): no gather, and the x or h tile is the same for every
+//     expert; 16 or 32 columns cost the tensor core nothing beside the stream.
+//   - Work is cut into K stages, not tiles: the gate / up phase has (expert,
+//     128 rows, stage) units, the down phase (128 rows, expert, stage) ones,
+//     and every CTA takes an equal run of them, whatever the routing.  Tiles
+//     that several CTAs share are summed by the last of them to finish, from
+//     fp32 partial tiles in the workspace, in the order of the K stages --
+//     the same order whoever is last, so results do not depend on timing.
+//   - A grid barrier separates the phases (cooperative launch: all CTAs are
+//     resident).  The producer fills the ring with the down phase's first
+//     weights before it waits there, so the stream goes on over the barrier.
+//   - Routing weights multiply the down products in fp32, expert by expert, as
+//     they leave TMEM; h stays unscaled.
+//
+// Roles (192 threads) as in the grouped kernel: warp 0 TMA producer, warp 1
+// MMA issuer, warps 2-5 epilogue; before that all warps compute the router.
+// Every wait is bounded; one that gives up records a status bit and its role
+// stops, the others then give up in turn, TMEM is freed.
+#pragma once
+#include "int8_rows.cuh"
+#include "spmm24_common.cuh"
+
+namespace spmm24 {
+
+constexpr int kMoeMaxTokens = 32;
+constexpr int kMoeMaxExperts = 256;
+constexpr int kMoeMaxTopK = 16;
+constexpr int kMoeMaxCtas = 160;
+constexpr int kMoeMaxTiles = 32768;     // (expert, 128 rows of I) tiles of the gate / up phase
+constexpr int kMoeMaxDownTiles = 4096;  // 128-row tiles of H
+constexpr int kMoeWarps = kThreads / 32;
+
+struct MoeParams {
+    CUtensorMap tmGU, tmGUE;  // gate and up weights of all experts: values, metadata
+    CUtensorMap tmD, tmDE;    // down weights
+    CUtensorMap tmX, tmH;     // the products' B operands: x (int8: its rounded rows), h
+    const uint16_t* x;        // packed strips
+    const uint16_t* router;   // E x H, or null: ids and weights are given
+    int* ids;                 // T x k
+    float* weights;
+    const float* gu_scale;    // int8: E x 2I, E x H
+    const float* d_scale;
+    uint16_t* y;
+    Epilogue epi;             // M = H, N = T
+    int T, H, I, E, k;
+    int strips;               // ceil(T / 8)
+    int act, norm, bf16;
+    int max_slots;            // min(E, T k): experts that can be in use
+    int logit_shares;         // K shares of a logit
+    // workspace
+    uint32_t* bar;            // arrivals, generation
+    uint32_t* tile_count;     // gate / up tiles, then down tiles; zero between launches
+    float* logits;            // [share][T][E]
+    float* part;              // [CTA][2][N_TILE / 2 quads][128 rows][4]
+    uint32_t* amax;           // int8: [slot][32] largest |h| (bits)
+    float* xscale;            // int8: [32]
+    int8_t* xq;               // int8: T x H
+    float* h32;               // int8: [slot][T][I]
+    int8_t* hq;               // int8: [slot][T][I]
+    uint16_t* h16;            // 16-bit: [slot][strips][I][8]
+};
+
+constexpr int moe_stages(int n_tile, bool i8) { return n_tile == 16 ? 9 : i8 ? 7 : 8; }
+
+template <int N_TILE, bool I8>
+struct MoeCfg : Cfg<N_TILE, moe_stages(N_TILE, I8), 4, I8> {
+    static constexpr int STAGES = moe_stages(N_TILE, I8);
+    using B_ = Cfg<N_TILE, STAGES, 4, I8>;
+    static constexpr int BAR_OFFSET = B_::RING_BYTES;
+    static constexpr int NUM_BARS = 2 * STAGES + 4;  // full, empty, acc_full[2], acc_empty[2]
+    static constexpr int AUX_OFFSET = (BAR_OFFSET + NUM_BARS * 8 + 15) / 16 * 16;
+    static constexpr int SMEM_BYTES = AUX_OFFSET + 6144;
+    static constexpr int SMEM_ALLOC = SMEM_BYTES + 1024;  // slack to align the base to 1024 B
+    static_assert(SMEM_ALLOC <= 232448, "shared memory overflow");
+    static_assert(B_::STAGE_BYTES % 1024 == 0, "stages must stay 1024-byte aligned");
+};
+
+// Routing and small state in shared memory.
+struct MoeShared {
+    int ids[kMoeMaxTokens * kMoeMaxTopK];        // -1: no expert
+    float weights[kMoeMaxTokens * kMoeMaxTopK];
+    uint32_t mask[kMoeMaxExperts];               // tokens of each expert
+    uint16_t list[kMoeMaxExperts];               // experts in use, in increasing order
+    float xscale[kMoeMaxTokens];
+    uint32_t red[kMoeWarps][8];
+    uint32_t top[8];
+    uint32_t tmem, gen0, n_active, last, dead;
+};
+static_assert(sizeof(MoeShared) <= 6144, "MoeCfg reserves 6 KB");
+
+// ------------------------------------------------------------ grid barrier
+// One arrival per CTA; the last one resets the count and starts the next
+// generation.  gen0 is the generation read before the CTA's first arrival, so
+// the launch's n-th barrier is over once the generation has passed gen0 + n.
+__device__ __forceinline__ void moe_arrive(uint32_t* bar, uint32_t ctas) {
+    __threadfence();
+    if (atomicAdd(bar, 1u) == ctas - 1u) {
+        bar[0] = 0u;
+        __threadfence();
+        atomicAdd(bar + 1, 1u);
+    }
+}
+__device__ __forceinline__ bool moe_wait(const uint32_t* bar, uint32_t gen) {
+    const uint64_t t0 = ptx::globaltimer();
+    uint32_t spins = 0;
+    while ((int)(ptx::ld_acquire_gpu(bar + 1) - gen) < 0) {
+        if ((++spins & 255u) == 0u && ptx::globaltimer() - t0 > kWaitLimitNs) {
+            atomicOr(&g_spmm24_status, kStatusBarrierTimeout);
+            return false;
+        }
+    }
+    return true;
+}
+
+// An equal run of the units 0 .. U - 1 for each of `ctas` CTAs (ctas <= U).
+__device__ __forceinline__ int moe_begin(int units, int cta, int ctas) { return (int)((long long)units * cta / ctas); }
+__device__ __forceinline__ int moe_owner(int units, int unit, int ctas) {
+    return (int)((((long long)unit + 1) * ctas - 1) / units);
+}
+
+// SiLU and GELU (tanh form, as y sigmoid(2 z)) to fp32 accuracy: the few
+// values of this layer are no load, and h is rounded after them.
+__device__ __forceinline__ float moe_activate(float y, int act) {
+    if (act == kActRelu) return y > 0.f || y != y ? y : 0.f;
+    if (act == kActSilu) return y / (1.f + __expf(-y));
+    if (act == kActGelu) return y / (1.f + __expf(-1.5957691216057308f * (y + 0.044715f * y * y * y)));
+    return y;
+}
+
+// ------------------------------------------------------------------ router
+// Unit (expert, strip of eight tokens, K share): one warp, eight partial
+// logits.  A lane takes eight consecutive inputs at a time.
+template <bool BF16>
+__device__ __forceinline__ void moe_router(const MoeParams& p, int unit0, int step, int lane) {
+    const int shares = p.logit_shares, groups = p.H / 8, per = (groups + shares - 1) / shares;
+    const int units = p.E * p.strips * shares;
+    for (int it = unit0; it < units; it += step) {
+        const int ks = it % shares, s = it / shares % p.strips, e = it / shares / p.strips;
+        const uint4* wrow = reinterpret_cast<const uint4*>(p.router + (size_t)e * p.H);
+        const uint4* xs = reinterpret_cast<const uint4*>(p.x) + (size_t)s * p.H;
+        float acc[8];
+#pragma unroll
+        for (int t = 0; t < 8; ++t) acc[t] = 0.f;
+        const int g1 = min(groups, (ks + 1) * per);
+        for (int g = ks * per + lane; g < g1; g += 32) {
+            const uint4 w4 = wrow[g];
+            uint4 xv[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) xv[i] = xs[8 * g + i];
+            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float w0, w1;
+                unpack2<BF16>(w[i >> 1], w0, w1);
+                const float wi = i & 1 ? w1 : w0;
+                const uint32_t xw[4] = {xv[i].x, xv[i].y, xv[i].z, xv[i].w};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    float a, b;
+                    unpack2<BF16>(xw[q], a, b);
+                    acc[2 * q] = fmaf(wi, a, acc[2 * q]);
+                    acc[2 * q + 1] = fmaf(wi, b, acc[2 * q + 1]);
+                }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+#pragma unroll
+            for (int o = 16; o; o >>= 1) acc[t] += __shfl_xor_sync(0xffffffffu, acc[t], o);
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+            if (lane == t && 8 * s + t < p.T) p.logits[((size_t)ks * p.T + 8 * s + t) * p.E + e] = acc[t];
+    }
+}
+
+// Top k of one token's logits and their weights; one warp.  Keys order as the
+// logits do, NaN above all (it then makes every weight NaN).
+__device__ __forceinline__ void moe_top_k(const MoeParams& p, MoeShared& sh, int t, int lane, bool publish) {
+    float l[kMoeMaxExperts / 32];
+    uint32_t key[kMoeMaxExperts / 32];
+#pragma unroll
+    for (int i = 0; i < kMoeMaxExperts / 32; ++i) {
+        const int e = lane + 32 * i;
+        l[i] = 0.f;
+        key[i] = 0u;
+        if (e < p.E) {
+            float v = 0.f;
+            for (int s = 0; s < p.logit_shares; ++s) v += __ldcg(p.logits + ((size_t)s * p.T + t) * p.E + e);
+            l[i] = v;
+            const uint32_t b = __float_as_uint(v + 0.f);  // -0 -> +0: the two are a tie
+            key[i] = v != v ? 0xffffffffu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
+        }
+    }
+    int my_id = -1;
+    float my_l = 0.f;
+    for (int j = 0; j < p.k; ++j) {
+        uint32_t best = 0u;
+        int bi = 0;
+        float bl = 0.f;
+#pragma unroll
+        for (int i = 0; i < kMoeMaxExperts / 32; ++i)
+            if (key[i] > best) {
+                best = key[i];
+                bi = i;
+                bl = l[i];
+            }
+        const uint32_t m = __reduce_max_sync(0xffffffffu, best);
+        const uint32_t win = __reduce_min_sync(0xffffffffu, best == m ? (uint32_t)(lane + 32 * bi) : 0xffffffffu);
+        const float lw = __shfl_sync(0xffffffffu, bl, (int)(win & 31u));
+        if (lane == (int)(win & 31u)) {
+#pragma unroll
+            for (int i = 0; i < kMoeMaxExperts / 32; ++i)
+                if (i == (int)(win >> 5)) key[i] = 0u;
+        }
+        if (lane == j) {
+            my_id = (int)win;
+            my_l = lw;
+        }
+    }
+    const float top = __shfl_sync(0xffffffffu, my_l, 0);
+    float sum = 0.f;
+    if (p.norm) {
+        sum = lane < p.k ? expf(my_l - top) : 0.f;
+    } else {
+#pragma unroll
+        for (int i = 0; i < kMoeMaxExperts / 32; ++i)
+            if (lane + 32 * i < p.E) sum += expf(l[i] - top);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane < p.k) {
+        const float w = expf(my_l - top) / sum;
+        sh.ids[t * p.k + lane] = my_id;
+        sh.weights[t * p.k + lane] = w;
+        if (publish) {
+            if (p.ids) p.ids[t * p.k + lane] = my_id;
+            if (p.weights) p.weights[t * p.k + lane] = w;
+        }
+    }
+}
+
+// int8: x -> int8 rows.  Unit (strip, one of `parts` column ranges): a block.
+// Every block finds its strip's eight maxima (the strip comes out of L2), then
+// rounds its own columns.
+template <bool BF16>
+__device__ __forceinline__ void moe_quantize_x(const MoeParams& p, MoeShared& sh, int unit, int parts) {
+    const int s = unit / parts, part = unit % parts, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint4* strip = reinterpret_cast<const uint4*>(p.x) + (size_t)s * p.H;
+    const uint32_t abs2 = 0x7fff7fffu;
+    uint32_t m[4] = {0u, 0u, 0u, 0u};
+#pragma unroll 4
+    for (int c = threadIdx.x; c < p.H; c += kThreads) {
+        const uint4 v = strip[c];
+        m[0] = vmaxu2(m[0], v.x & abs2);
+        m[1] = vmaxu2(m[1], v.y & abs2);
+        m[2] = vmaxu2(m[2], v.z & abs2);
+        m[3] = vmaxu2(m[3], v.w & abs2);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t lo = __reduce_max_sync(0xffffffffu, m[i] & 0xffffu);
+        const uint32_t hi = __reduce_max_sync(0xffffffffu, m[i] >> 16);
+        if (lane == 0) {
+            sh.red[warp][2 * i] = lo;
+            sh.red[warp][2 * i + 1] = hi;
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x < 8) {
+        uint32_t t = 0u;
+        for (int w = 0; w < kMoeWarps; ++w) t = max(t, sh.red[w][threadIdx.x]);
+        sh.top[threadIdx.x] = t;
+        const int row = 8 * s + (int)threadIdx.x;
+        if (part == 0 && row < p.T) row_scale<BF16>(t, p.xscale + row);
+    }
+    __syncthreads();
+    const int groups = p.H / 8, g1 = (int)((long long)groups * (part + 1) / parts);
+    for (int g = (int)((long long)groups * part / parts) + threadIdx.x; g < g1; g += kThreads) {
+        uint4 v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = strip[8 * g + i];
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+            if (8 * s + t >= p.T) break;
+            const RowScale r = row_scale<BF16>(sh.top[t], nullptr);
+            uint32_t q[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t w = t < 2 ? v[i].x : t < 4 ? v[i].y : t < 6 ? v[i].z : v[i].w;
+                float a, b;
+                unpack2<BF16>(w, a, b);
+                q[i] = r.live ? quantize<BF16>(t & 1 ? b : a, r) : 0u;
+            }
+            *reinterpret_cast<uint2*>(p.xq + (size_t)(8 * s + t) * p.H + 8 * g) =
+                make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
+        }
+    }
+    __syncthreads();  // sh.red and sh.top are free again
+}
+
+// ------------------------------------------------------------------ stages
+template <class C_>
+__device__ __forceinline__ void moe_load_acts(uint8_t* st, uint64_t* bar, const CUtensorMap* tm, int slot, int strips,
+                                              int s, uint64_t pol) {
+    if constexpr (C_::kFp8) {  // rows [slot][token] of int8: two boxes of 128 bytes x N_TILE rows
+        ptx::tma_load_3d(st + C_::A_BYTES, tm, bar, 256 * s, 0, slot, pol);
+        ptx::tma_load_3d(st + C_::A_BYTES + C_::B_BYTES / 2, tm, bar, 256 * s + 128, 0, slot, pol);
+    } else {
+        ptx::tma_load_4d(st + C_::A_BYTES, tm, bar, 0, 2 * s, 0, slot * strips, pol);
+    }
+}
+
+// The four sparse MMAs of one stage (mma_stage, mma_stage_fp8), with the
+// activations of another slot of the ring: the up product reads the gate
+// product's.
+template <class C_, int N_TILE, bool I8>
+__device__ __forceinline__ void moe_mma_stage(uint32_t st, uint32_t st_acts, uint32_t meta_col, uint32_t d_tmem,
+                                              uint32_t accumulate, uint32_t fmt) {
+    const uint32_t stB = st_acts + C_::A_BYTES, stE = st + C_::A_BYTES + C_::B_BYTES;
+    ptx::tmem_cp_128x128b(meta_col, smem_desc(stE, 0, 128));
+    if constexpr (I8) {
+        constexpr uint32_t idesc = (make_idesc_fp8<N_TILE>() & ~kIdescF32) | kIdescInt8;
+        ptx::tmem_cp_128x128b(meta_col + 4, smem_desc(stE + 2048, 0, 128));
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            ptx::mma_sp_i8(d_tmem, smem_desc(st + j * 4096, 2048, 128),
+                           smem_desc_sw128(stB + (j >> 1) * (C_::B_BYTES / 2) + (j & 1) * 64), meta_col + 2 * j, idesc,
+                           j ? 1u : accumulate);
+    } else {
+        const uint32_t idesc = make_idesc<N_TILE>() | fmt;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            ptx::mma_sp_f16(d_tmem, smem_desc(st + j * 2048, 4 * 2048, 128), smem_desc(stB + j * 512, 128, 2048),
+                            meta_col + (j & 2), idesc | (uint32_t)(j & 1), j ? 1u : accumulate);
+    }
+}
+
+template <int N_TILE>
+__device__ __forceinline__ void moe_read_acc(uint32_t taddr, uint32_t (&v)[N_TILE]) {
+#pragma unroll
+    for (int c = 0; c < N_TILE; c += 16) ptx::tmem_ld_32x32b_x16(taddr + c, *reinterpret_cast<uint32_t(*)[16]>(v + c));
+}
+
+template <bool I8>
+__device__ __forceinline__ uint32_t moe_add(uint32_t a, uint32_t b) {
+    return I8 ? a + b : __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+}
+
+// A tile that several CTAs share: this CTA's partial (NV words per row, the
+// first 4 tq of every N_TILE of them in use) goes to the workspace; the last
+// CTA to get here adds all partials in K order into v and returns true.
+// INT: the words are 32-bit integers.  Called by the 128 epilogue threads.
+template <int N_TILE, int NV, bool INT>
+__device__ __forceinline__ bool moe_share_tile(const MoeParams& p, MoeShared& sh, uint32_t (&v)[NV], int row, int units,
+                                               int ctas, int tile, int stages, uint32_t* count) {
+    constexpr int SLOT = kTileM * 2 * N_TILE;  // floats of one partial
+    const int tq = (p.T + 3) / 4, first = tile * stages;
+    const int c0 = moe_owner(units, first, ctas), c1 = moe_owner(units, first + stages - 1, ctas);
+    const int me = (int)blockIdx.x;
+    // A CTA's run touches a shared tile with its first segment (slot 0) or its last (slot 1).
+    auto base = [&](int c) {
+        return reinterpret_cast<uint4*>(p.part + ((size_t)c * 2 + (moe_begin(units, c, ctas) < first ? 1 : 0)) * SLOT) + row;
+    };
+    uint4* own = base(me);
+#pragma unroll
+    for (int q = 0; q < NV / 4; ++q)
+        if (q % (N_TILE / 4) < tq)
+            __stcg(own + (size_t)q * kTileM, make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]));
+    __threadfence();
+    ptx::named_barrier(kBarEpi, kEpiThreads);
+    if (threadIdx.x == 64) {
+        const bool last = atomicAdd(count + tile, 1u) == (uint32_t)(c1 - c0);
+        if (last) count[tile] = 0u;  // for the next launch
+        sh.last = last ? 1u : 0u;
+        __threadfence();
+    }
+    ptx::named_barrier(kBarEpi, kEpiThreads);
+    const bool last = sh.last != 0u;
+    ptx::named_barrier(kBarEpi, kEpiThreads);  // sh.last may be written again
+    if (!last) return false;
+    __threadfence();
+#pragma unroll
+    for (int i = 0; i < NV; ++i) v[i] = 0u;
+    for (int c = c0; c <= c1; ++c) {
+        const uint4* b = base(c);
+#pragma unroll
+        for (int q = 0; q < NV / 4; ++q)
+            if (q % (N_TILE / 4) < tq) {
+                const uint4 x = __ldcg(b + (size_t)q * kTileM);
+                v[4 * q] = moe_add<INT>(v[4 * q], x.x);
+                v[4 * q + 1] = moe_add<INT>(v[4 * q + 1], x.y);
+                v[4 * q + 2] = moe_add<INT>(v[4 * q + 2], x.z);
+                v[4 * q + 3] = moe_add<INT>(v[4 * q + 3], x.w);
+            }
+    }
+    return true;
+}
+
+template <int N_TILE, bool I8>
+__global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_constant__ MoeParams p) {
+    using C_ = MoeCfg<N_TILE, I8>;
+    constexpr int STAGES = C_::STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C_::BAR_OFFSET);
+    uint64_t* empty = full + STAGES;
+    uint64_t* acc_full = empty + STAGES;  // [2]
+    uint64_t* acc_empty = acc_full + 2;   // [2]
+    MoeShared& sh = *reinterpret_cast<MoeShared*>(smem + C_::AUX_OFFSET);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int cta = (int)blockIdx.x, grid = (int)gridDim.x;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            ptx::mbar_init(&full[s], 1);
+            ptx::mbar_init(&empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            ptx::mbar_init(&acc_full[b], 1);
+            ptx::mbar_init(&acc_empty[b], kEpiThreads / 32);
+        }
+        ptx::fence_mbarrier_init();
+        sh.gen0 = ptx::ld_acquire_gpu(p.bar + 1);  // before this CTA's first arrival
+        sh.dead = 0u;
+        ptx::prefetch_tmap(&p.tmGU);
+        ptx::prefetch_tmap(&p.tmGUE);
+        ptx::prefetch_tmap(&p.tmX);
+        ptx::prefetch_tmap(&p.tmD);
+        ptx::prefetch_tmap(&p.tmDE);
+        ptx::prefetch_tmap(&p.tmH);
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc(&sh.tmem, C_::TMEM_COLS);
+        ptx::tmem_relinquish();
+    }
+    for (int e = threadIdx.x; e < kMoeMaxExperts; e += kThreads) sh.mask[e] = 0u;
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem_base = sh.tmem;
+
+    // ------------------------------------------- router, rounding of x
+    int quant_ctas = 0;
+    if constexpr (I8) {
+        const int parts = min(8, max(1, grid / 2 / p.strips));
+        quant_ctas = p.strips * parts;
+        for (int u = cta; u < quant_ctas; u += grid) {
+            if (p.bf16) moe_quantize_x<true>(p, sh, u, parts);
+            else moe_quantize_x<false>(p, sh, u, parts);
+        }
+        if (cta == grid - 1)  // the largest |h| of this launch starts from zero
+            for (int i = threadIdx.x; i < p.max_slots * kMoeMaxTokens; i += kThreads) p.amax[i] = 0u;
+    }
+    if (p.router) {
+        // the CTAs that do not round x come first
+        const int unit0 = ((cta + grid - quant_ctas % grid) % grid) * kMoeWarps + warp;
+        if (p.bf16) moe_router<true>(p, unit0, grid * kMoeWarps, lane);
+        else moe_router<false>(p, unit0, grid * kMoeWarps, lane);
+    }
+    uint32_t gen = sh.gen0;
+    if (I8 || p.router) {
+        if constexpr (I8) ptx::fence_proxy_async_global();  // xq is read by TMA
+        __syncthreads();
+        ++gen;
+        if (threadIdx.x == 0) {
+            moe_arrive(p.bar, (uint32_t)grid);
+            if (!moe_wait(p.bar, gen)) sh.dead = 1u;
+            __threadfence();
+        }
+        __syncthreads();
+    }
+
+    // --------------------------------------------------------- routing
+    if (p.router) {
+        for (int t = warp; t < p.T; t += kMoeWarps) moe_top_k(p, sh, t, lane, cta == 0);
+    } else {
+        for (int i = threadIdx.x; i < p.T * p.k; i += kThreads) {
+            const int e = p.ids[i];
+            sh.ids[i] = e >= 0 && e < p.E ? e : -1;
+            sh.weights[i] = p.weights[i];
+        }
+    }
+    if (I8 && threadIdx.x < p.T) sh.xscale[threadIdx.x] = __ldcg(p.xscale + threadIdx.x);
+    __syncthreads();
+    for (int i = threadIdx.x; i < p.T * p.k; i += kThreads)
+        if (sh.ids[i] >= 0) atomicOr(&sh.mask[sh.ids[i]], 1u << (i / p.k));
+    __syncthreads();
+    if (warp == 0) {
+        int n = 0;
+        for (int e0 = 0; e0 < p.E; e0 += 32) {
+            const bool used = e0 + lane < p.E && sh.mask[e0 + lane] != 0u;
+            const uint32_t b = __ballot_sync(0xffffffffu, used);
+            if (used) sh.list[n + __popc(b & ((1u << lane) - 1u))] = (uint16_t)(e0 + lane);
+            n += __popc(b);
+        }
+        if (lane == 0) sh.n_active = (uint32_t)n;
+    }
+    __syncthreads();
+
+    const int n_active = sh.dead ? 0 : (int)sh.n_active;
+    const int stage_k = I8 ? 256 : 128;
+    const int gu_groups = p.H * 2 / stage_k, d_groups = p.I * 2 / stage_k;  // metadata groups along K
+    const int S1 = (gu_groups + 1) / 2, Se = (d_groups + 1) / 2;            // stages of one gate / up, one down product
+    const int i_tiles = (p.I + kTileM - 1) / kTileM, h_tiles = (p.H + kTileM - 1) / kTileM;
+    // gate / up: unit (slot, 128 rows of I, stage); down: unit (128 rows of H, slot, stage)
+    const int U1 = n_active * i_tiles * S1, S2 = n_active * Se, U2 = h_tiles * S2;
+    const int G1 = min(grid, U1), G2 = min(grid, U2);
+    const int b1 = cta < G1 ? moe_begin(U1, cta, G1) : 0, e1 = cta < G1 ? moe_begin(U1, cta + 1, G1) : 0;
+    const int b2 = cta < G2 ? moe_begin(U2, cta, G2) : 0, e2 = cta < G2 ? moe_begin(U2, cta + 1, G2) : 0;
+    const uint32_t gen_h = gen + (I8 ? 2u : 1u);  // h (int8: rounded) is complete
+
+    if (warp == 0) {
+        // ------------------------------------------------ TMA producer
+        if (lane == 0 && n_active > 0) {
+            const uint64_t pol_stream = ptx::policy_evict_first(), pol_keep = ptx::policy_evict_last();
+            const uint32_t acts_bytes = I8 ? C_::B_BYTES : (uint32_t)p.strips * 2048u;
+            const uint32_t w_bytes = C_::A_BYTES + C_::E_BYTES;
+            if constexpr (I8) ptx::fence_proxy_async_global();
+            int it = 0, issued = 0;  // ring slots used by the gate / up phase; armed in all
+            bool ok = true;
+            auto slot_of = [&](int i) { return i % STAGES; };
+            auto acquire = [&](int i, uint32_t bytes) {
+                const int s = slot_of(i);
+                if (i >= STAGES && !ptx::mbar_wait_bounded(&empty[s], (uint32_t)(i / STAGES - 1) & 1u, kWaitLimitNs)) {
+                    atomicOr(&g_spmm24_status, kStatusProducerTimeout);
+                    return false;
+                }
+                ptx::mbar_arrive_expect_tx(&full[s], bytes);
+                issued = i + 1;
+                return true;
+            };
+            for (int u = b1; u < e1 && ok; ++u) {
+                const int tile = u / S1, s = u % S1;
+                const int e = sh.list[tile / i_tiles], row0 = e * 2 * p.I + tile % i_tiles * kTileM;
+                for (int half = 0; half < 2 && ok; ++half, ++it) {
+                    ok = acquire(it, half ? w_bytes : w_bytes + acts_bytes);
+                    if (!ok) break;
+                    uint8_t* st = smem + slot_of(it) * C_::STAGE_BYTES;
+                    load_stage_weights<C_>(st, &full[slot_of(it)], &p.tmGU, &p.tmGUE, (row0 + half * p.I) / 16, 2 * s,
+                                           pol_stream);
+                    if (!half) moe_load_acts<C_>(st, &full[slot_of(it)], &p.tmX, 0, p.strips, s, pol_keep);
+                }
+            }
+            // The down phase: the first stages' weights before the wait for h.
+            auto weights2 = [&](int u, int i) {
+                const int tile = u / S2, s = u % S2;
+                load_stage_weights<C_>(smem + slot_of(i) * C_::STAGE_BYTES, &full[slot_of(i)], &p.tmD, &p.tmDE,
+                                       (sh.list[s / Se] * p.H + tile * kTileM) / 16, 2 * (s % Se), pol_stream);
+            };
+            auto acts2 = [&](int u, int i) {
+                const int s = u % S2;
+                moe_load_acts<C_>(smem + slot_of(i) * C_::STAGE_BYTES, &full[slot_of(i)], &p.tmH, s / Se, p.strips,
+                                  s % Se, pol_keep);
+            };
+            int ahead = 0;
+            while (ok && ahead < STAGES && b2 + ahead < e2) {
+                ok = acquire(it + ahead, w_bytes + acts_bytes);
+                if (ok) {
+                    weights2(b2 + ahead, it + ahead);
+                    ++ahead;
+                }
+            }
+            if (ok && b2 < e2) {
+                ok = moe_wait(p.bar, gen_h);
+                ptx::fence_proxy_async_global();
+                if (ok) {
+                    for (int i = 0; i < ahead; ++i) acts2(b2 + i, it + i);
+                    for (int i = ahead; b2 + i < e2 && ok; ++i) {
+                        if (!(ok = acquire(it + i, w_bytes + acts_bytes))) break;
+                        weights2(b2 + i, it + i);
+                        acts2(b2 + i, it + i);
+                    }
+                }
+            }
+            if (!ok)  // gave up: let the copies in flight land before the block ends
+                for (int i = max(0, issued - STAGES); i < issued; ++i)
+                    ptx::mbar_wait_bounded(&full[slot_of(i)], (uint32_t)(i / STAGES) & 1u, 10000000ull);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // -------------------------------------------------- MMA issuer
+        const uint32_t smem_base = ptx::smem_u32(smem), fmt = p.bf16 ? kIdescBf16 : 0u;
+        int it = 0, j = 0;
+        bool ok = true;
+        // waits until accumulator pair j & 1 has been read; false: give up
+        auto begin_acc = [&]() {
+            if (j >= 2) {
+                if (!__all_sync(0xffffffffu, ptx::mbar_wait_bounded(&acc_empty[j & 1], (uint32_t)((j >> 1) - 1) & 1u,
+                                                                    kWaitLimitNs))) {
+                    if (lane == 0) atomicOr(&g_spmm24_status, kStatusMmaTimeout);
+                    return false;
+                }
+                ptx::tc_fence_after();
+            }
+            return true;
+        };
+        auto wait_full = [&](int i) {
+            if (!__all_sync(0xffffffffu, ptx::mbar_wait_bounded(&full[i % STAGES], (uint32_t)(i / STAGES) & 1u,
+                                                                kWaitLimitNs))) {
+                if (lane == 0) atomicOr(&g_spmm24_status, kStatusMmaTimeout);
+                return false;
+            }
+            ptx::tc_fence_after();
+            return true;
+        };
+        auto stage = [&](int i, int acts, uint32_t d, uint32_t accumulate) {
+            moe_mma_stage<C_, N_TILE, I8>(smem_base + i % STAGES * C_::STAGE_BYTES,
+                                          smem_base + acts % STAGES * C_::STAGE_BYTES,
+                                          tmem_base + C_::META_COL + C_::META_STRIDE * (i % STAGES), d, accumulate, fmt);
+        };
+        for (int u = b1; u < e1 && ok;) {
+            const int s0 = u % S1, s1 = min(S1, s0 + e1 - u);
+            if (!(ok = begin_acc())) break;
+            const uint32_t d = tmem_base + (uint32_t)((j & 1) * 2 * N_TILE);
+            for (int s = s0; s < s1 && ok; ++s, it += 2) {
+                for (int half = 0; half < 2; ++half) {
+                    if (!(ok = wait_full(it + half))) break;
+                    if (2 * s + 1 >= gu_groups)
+                        patch_tail_metadata<C_>(smem + (it + half) % STAGES * C_::STAGE_BYTES, lane);
+                    if (lane == 0) {
+                        stage(it + half, it, d + (uint32_t)(half * N_TILE), s > s0);
+                        if (half) {  // the up product was the last to read the gate slot's activations
+                            ptx::tc_commit(&empty[it % STAGES]);
+                            ptx::tc_commit(&empty[(it + 1) % STAGES]);
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+            if (!ok) break;
+            if (lane == 0) ptx::tc_commit(&acc_full[j & 1]);
+            __syncwarp();
+            ++j;
+            u += s1 - s0;
+        }
+        for (int u = b2; u < e2 && ok;) {  // a segment ends with its expert: the epilogue weighs each on its own
+            const int s0 = u % Se, s1 = min(Se, s0 + e2 - u);
+            if (!(ok = begin_acc())) break;
+            const uint32_t d = tmem_base + (uint32_t)((j & 1) * 2 * N_TILE);
+            for (int s = s0; s < s1; ++s, ++it) {
+                if (!(ok = wait_full(it))) break;
+                if (2 * s + 1 >= d_groups) patch_tail_metadata<C_>(smem + it % STAGES * C_::STAGE_BYTES, lane);
+                if (lane == 0) {
+                    stage(it, it, d, s > s0);
+                    ptx::tc_commit(&empty[it % STAGES]);
+                }
+                __syncwarp();
+            }
+            if (!ok) break;
+            if (lane == 0) ptx::tc_commit(&acc_full[j & 1]);
+            __syncwarp();
+            ++j;
+            u += s1 - s0;
+        }
+    } else {
+        // ---------------------------------------------------- epilogue
+        const int quad = warp & 3, row = quad * 32 + lane;  // thread = output row (TMEM lane)
+        const uint32_t tmem_row = tmem_base + ((uint32_t)(quad * 32) << 16);
+        int j = 0;
+        bool ok = true;
+        // A warp whose wait gave up goes on without waiting, so that the warps
+        // still meet at their barriers (the launch's outputs are then void).
+        auto wait_acc = [&]() {
+            if (ok && !__all_sync(0xffffffffu, ptx::mbar_wait_bounded(&acc_full[j & 1], (uint32_t)(j >> 1) & 1u,
+                                                                      kWaitLimitNs))) {
+                atomicOr(&g_spmm24_status, kStatusEpilogueTimeout);
+                ok = false;
+            }
+            ptx::tc_fence_after();
+        };
+        auto release_acc = [&]() {
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&acc_empty[j & 1]);
+            ++j;
+        };
+        for (int u = b1; u < e1;) {
+            const int tile = u / S1, s0 = u % S1, s1 = min(S1, s0 + e1 - u);
+            u += s1 - s0;
+            uint32_t v[2 * N_TILE];  // gate, up
+            wait_acc();
+            moe_read_acc<2 * N_TILE>(tmem_row + (uint32_t)((j & 1) * 2 * N_TILE), v);
+            ptx::tmem_wait_ld();
+            release_acc();
+            if (s1 - s0 < S1 &&
+                !moe_share_tile<N_TILE, 2 * N_TILE, I8>(p, sh, v, row, U1, G1, tile, S1, p.tile_count))
+                continue;
+            const int slot = tile / i_tiles, e = sh.list[slot], r = tile % i_tiles * kTileM + row;
+            const bool live = r < p.I;
+            if constexpr (I8) {
+                const float gs = live ? p.gu_scale[(size_t)e * 2 * p.I + r] : 0.f;
+                const float us = live ? p.gu_scale[(size_t)e * 2 * p.I + p.I + r] : 0.f;
+                const uint32_t mask = sh.mask[e];
+#pragma unroll
+                for (int t = 0; t < N_TILE; ++t) {
+                    if (!(mask >> t & 1u)) continue;
+                    const float xs = sh.xscale[t];
+                    const float h = live ? moe_activate(int8_value((int)v[t], gs, xs), p.act) *
+                                               int8_value((int)v[N_TILE + t], us, xs)
+                                         : 0.f;
+                    if (live) __stcg(p.h32 + ((size_t)slot * p.T + t) * p.I + r, h);
+                    // bits order as magnitudes, NaN above all
+                    const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(h) & 0x7fffffffu);
+                    if (lane == 0) atomicMax(p.amax + slot * kMoeMaxTokens + t, m);
+                }
+            } else if (live) {
+#pragma unroll
+                for (int s = 0; s < N_TILE / 8; ++s) {
+                    if (s >= p.strips) break;
+                    uint32_t w[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int t = 8 * s + 2 * q;
+                        w[q] = pack2(moe_activate(__uint_as_float(v[t]), p.act) * __uint_as_float(v[N_TILE + t]),
+                                     moe_activate(__uint_as_float(v[t + 1]), p.act) * __uint_as_float(v[N_TILE + t + 1]),
+                                     p.bf16);
+                    }
+                    *reinterpret_cast<uint4*>(p.h16 + (((size_t)slot * p.strips + s) * p.I + r) * 8) =
+                        make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+        }
+        // h is in place: this CTA's share
+        if (n_active > 0) {
+            if constexpr (!I8) ptx::fence_proxy_async_global();  // h is read by TMA
+            __threadfence();
+            ptx::named_barrier(kBarEpi, kEpiThreads);
+            if (threadIdx.x == 64 && ok) moe_arrive(p.bar, (uint32_t)grid);
+        }
+        if constexpr (I8) {
+            if (n_active > 0) {
+                // round h: (slot, token) rows in pieces of 512 values, a block each
+                if (threadIdx.x == 64) sh.last = ok && moe_wait(p.bar, gen + 1u) ? 1u : 0u;
+                ptx::named_barrier(kBarEpi, kEpiThreads);
+                ok = ok && sh.last != 0u;
+                ptx::named_barrier(kBarEpi, kEpiThreads);
+                __threadfence();
+                {
+                    const int pieces = (p.I + 511) / 512, units = ok ? n_active * p.T * pieces : 0;
+                    for (int w = cta; w < units; w += grid) {
+                        const int piece = w % pieces, pair = w / pieces, slot = pair / p.T, t = pair % p.T;
+                        if (!(sh.mask[sh.list[slot]] >> t & 1u)) continue;
+                        const int c = piece * 512 + (threadIdx.x - 64) * 4;
+                        if (c >= p.I) continue;
+                        const float a = __uint_as_float(__ldcg(p.amax + slot * kMoeMaxTokens + t));
+                        const float inv = 127.f / a;
+                        // else the row is zero (or below 1e-36), infinite or NaN: zeros, times its scale
+                        const bool finite = inv > 0.f && inv <= 3.402823466e38f;
+                        const float4 h = __ldcg(reinterpret_cast<const float4*>(p.h32 + (size_t)pair * p.I + c));
+                        const float hv[4] = {h.x, h.y, h.z, h.w};
+                        uint32_t q[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) q[i] = finite ? (uint32_t)__float2int_rn(hv[i] * inv) : 0u;
+                        *reinterpret_cast<uint32_t*>(p.hq + (size_t)pair * p.I + c) = pack4(q[0], q[1], q[2], q[3]);
+                    }
+                    ptx::fence_proxy_async_global();  // hq is read by TMA
+                    __threadfence();
+                    ptx::named_barrier(kBarEpi, kEpiThreads);
+                    if (threadIdx.x == 64 && ok) moe_arrive(p.bar, (uint32_t)grid);
+                }
+            }
+        }
+        const bool vec = (p.T % 8 == 0) && ((reinterpret_cast<uintptr_t>(p.y) & 15u) == 0) &&
+                         ((reinterpret_cast<uintptr_t>(p.epi.residual) & 15u) == 0);
+        const bool plain = epilogue_is_plain(p.epi);
+        auto finish = [&](uint32_t (&y)[N_TILE], int tile) {
+            const int gm = tile * kTileM + row;
+            if (gm >= p.H) return;
+#pragma unroll
+            for (int c = 0; c < N_TILE; c += 8) {
+                if (c >= p.T) break;
+                float f[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(y[c + i]);
+                epilogue_store8(p.y, f, p.epi, gm, c, p.H, p.T, vec, plain);
+            }
+        };
+        for (int u = b2; u < e2;) {
+            const int tile = u / S2, s0 = u % S2, s1 = min(S2, s0 + e2 - u);
+            uint32_t y[N_TILE];
+#pragma unroll
+            for (int t = 0; t < N_TILE; ++t) y[t] = 0u;
+            for (int s = s0; s < s1;) {
+                const int slot = s / Se, e = sh.list[slot];
+                // this expert's weight of token `lane` (the same expert twice: the sum)
+                float w = 0.f, scale = 1.f;
+                const uint32_t mask = sh.mask[e];
+                if (lane < p.T)
+                    for (int i = 0; i < p.k; ++i)
+                        if (sh.ids[lane * p.k + i] == e) w += sh.weights[lane * p.k + i];
+                if constexpr (I8) {
+                    if (mask >> lane & 1u) w *= __uint_as_float(__ldcg(p.amax + slot * kMoeMaxTokens + lane)) / 127.f;
+                    const int gm = tile * kTileM + row;
+                    scale = gm < p.H ? p.d_scale[(size_t)e * p.H + gm] : 0.f;
+                }
+                uint32_t v[N_TILE];
+                wait_acc();
+                moe_read_acc<N_TILE>(tmem_row + (uint32_t)((j & 1) * 2 * N_TILE), v);
+                ptx::tmem_wait_ld();
+                release_acc();
+#pragma unroll
+                for (int t = 0; t < N_TILE; ++t) {
+                    const float wt = __shfl_sync(0xffffffffu, w, t);
+                    const float d = I8 ? (float)(int)v[t] * scale : __uint_as_float(v[t]);
+                    if (mask >> t & 1u) y[t] = __float_as_uint(fmaf(wt, d, __uint_as_float(y[t])));
+                }
+                s = min(s1, (slot + 1) * Se);
+            }
+            u += s1 - s0;
+            if (s1 - s0 < S2 &&
+                !moe_share_tile<N_TILE, N_TILE, false>(p, sh, y, row, U2, G2, tile, S2, p.tile_count + kMoeMaxTiles))
+                continue;
+            finish(y, tile);
+        }
+        if (n_active == 0 && !sh.dead) {  // no token has an expert
+            uint32_t y[N_TILE];
+#pragma unroll
+            for (int t = 0; t < N_TILE; ++t) y[t] = 0u;
+            for (int tile = cta; tile < h_tiles; tile += grid) finish(y, tile);
+        }
+    }
+
+    ptx::tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc(tmem_base, C_::TMEM_COLS);
+    }
+}
+
+}  // namespace spmm24

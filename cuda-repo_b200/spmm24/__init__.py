@@ -156,6 +156,7 @@ OUT_ROW_MAJOR, OUT_PACKED_B = 0, 1                    # SPMM24_OUT_*
 PRUNE_NONE, PRUNE_F16, PRUNE_BF16 = 0, 1, 2           # SPMM24_PRUNE_*
 FP8_E4M3, FP8_E5M2 = 0, 1                             # SPMM24_FP8_E4M3 / E5M2
 FP8_A_E5M2, FP8_B_E5M2 = 8, 16                        # spmm24_launch_fp8 flags
+MOE_INT8 = 32                                         # SPMM24_MOE_INT8 (spmm24_launch_moe)
 
 
 class SpmmError(RuntimeError):
@@ -256,6 +257,46 @@ def quantize_int8(x, rows: int, cols: int, q=None, scale=None, bf16: bool = Fals
     if rc != CUDA_SUCCESS:
         raise SpmmError(rc, "spmm24_quantize_int8")
     return q, scale
+
+
+class MoeLayer(ctypes.Structure):
+    """spmm24_moe_layer (include/spmm24/SpMM_API.h)."""
+    _fields_ = ([(n, ctypes.c_int) for n in ("tokens", "hidden", "inter", "experts", "top_k", "activation", "norm_topk")]
+                + [(n, ctypes.c_void_p) for n in
+                   ("x", "router", "gate_up", "gate_up_meta", "down", "down_meta", "gate_up_scale", "down_scale",
+                    "topk_ids", "topk_weights", "y", "epilogue", "workspace")]
+                + [("workspace_bytes", ctypes.c_size_t)])
+
+
+_lib.spmm24_launch_moe.argtypes = [_vp, ctypes.POINTER(MoeLayer), ctypes.c_uint]
+_lib.spmm24_launch_moe.restype = ctypes.c_int
+_lib.spmm24_moe_workspace_bytes.argtypes = [ctypes.c_int] * 5 + [ctypes.c_uint]
+_lib.spmm24_moe_workspace_bytes.restype = ctypes.c_size_t
+
+
+def moe_workspace_bytes(tokens: int, hidden: int, inter: int, experts: int, top_k: int, flags: int = 0) -> int:
+    """spmm24_moe_workspace_bytes: the workspace launch_moe needs for these sizes."""
+    n = int(_lib.spmm24_moe_workspace_bytes(tokens, hidden, inter, experts, top_k, flags))
+    if n == 0:
+        raise ValueError("sizes that spmm24_launch_moe does not take")
+    return n
+
+
+def launch_moe(stream, x, router, gate_up, gate_up_meta, down, down_meta, y, tokens: int, hidden: int, inter: int,
+               experts: int, top_k: int, workspace, flags: int = 0, gate_up_scale=None, down_scale=None, topk_ids=None,
+               topk_weights=None, activation: int = ACT_SILU, norm_topk: bool = True, bias=None, residual=None,
+               alpha: float = 1.0, epilogue_activation: int = ACT_NONE, out_layout: int = OUT_ROW_MAJOR) -> int:
+    """spmm24_launch_moe: a whole mixture-of-experts layer for 1..32 tokens in
+    one launch.  x: packed strips of tokens; workspace: a tensor of at least
+    moe_workspace_bytes bytes, zeroed once before its first use; the bias,
+    residual, alpha, epilogue_activation and out_layout of y as in
+    launch_fused.  Returns the cudaError_t code."""
+    epi = Epilogue(_ptr(bias), _ptr(residual), float(alpha), int(epilogue_activation), int(out_layout))
+    layer = MoeLayer(tokens, hidden, inter, experts, top_k, int(activation), int(norm_topk), _ptr(x), _ptr(router),
+                     _ptr(gate_up), _ptr(gate_up_meta), _ptr(down), _ptr(down_meta), _ptr(gate_up_scale),
+                     _ptr(down_scale), _ptr(topk_ids), _ptr(topk_weights), _ptr(y), ctypes.addressof(epi),
+                     _ptr(workspace), workspace.numel() * workspace.element_size())
+    return _lib.spmm24_launch_moe(_stream_handle(stream), ctypes.byref(layer), flags)
 
 
 class Problem(ctypes.Structure):

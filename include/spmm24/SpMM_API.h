@@ -417,6 +417,74 @@ cudaError_t spmm24_launch_int8(cudaStream_t stream, const void* values, const vo
                                int M, int N, int K, const float* w_scale, const float* x_scale, int split_k,
                                unsigned flags, const spmm24_epilogue* epilogue);
 
+/* ------------------------------------------------ mixture of experts
+ * A whole mixture-of-experts layer for a few tokens (a decode step) in one
+ * launch (no counterpart in the reference):
+ *     l[t, e] = sum_i router[e, i] x[t, i]                 (fp32 sums)
+ *     chosen  = the top_k largest l[t, .], largest first, ties to the lower
+ *               expert; a NaN counts as the largest
+ *     w[t, j] = softmax(l[t, .]) of the j-th chosen expert; norm_topk != 0:
+ *               divided by their sum over j
+ *     h       = act(Wgate_e x_t) * (Wup_e x_t)             e = the j-th chosen
+ *     y[:, t] = epilogue(sum_j w[t, j] Wdown_e h)
+ * Only the chosen experts' weights are read, each once.  16-bit experts
+ * (fp16; bf16 with SPMM24_BF16): h is rounded to the operand type.  int8
+ * experts (SPMM24_MOE_INT8): x_t is rounded to int8 as spmm24_quantize_int8
+ * rounds rows, every h likewise (scale max |h| / 127), sums are exact and
+ * scaled by channel and row; x, router and y stay 16-bit.
+ * The result does not depend on timing: the same call gives the same bits.
+ *
+ *   tokens      1..32 (T); hidden H and inter I: multiples of 64 (int8: 128);
+ *               experts 1..256 (E); top_k 1..min(E, 16);
+ *               min(E, T * top_k) * ceil(I / 128) <= 32768
+ *   x           packed B: ceil(T/8) strips of H x 8
+ *   router      E x H row-major 16-bit; or NULL: topk_ids and topk_weights
+ *               are inputs, an id outside 0..E-1 standing for no expert (a
+ *               padded token has none: its y is epilogue(0)), and an id that a
+ *               token names twice counting with the sum of its weights
+ *   gate_up     the experts one after another, each a packed 2I x H matrix,
+ *               gate rows first (packed matrices of the same K stack along M
+ *               by following one another); gate_up_meta: its metadata.  int8:
+ *               the 8-bit formats, and gate_up_scale holds E x 2I floats
+ *   down        likewise H x I for each expert; down_scale: E x H floats
+ *   activation  SPMM24_ACT_* of the gate
+ *   topk_ids    T x top_k int, topk_weights T x top_k float: outputs (either
+ *               may be NULL), or inputs without a router
+ *   y           H x T 16-bit (with an epilogue that says so, packed B);
+ *               epilogue as for spmm24_launch_fused with M = H, N = T, or NULL
+ *   workspace   spmm24_moe_workspace_bytes bytes, 256-byte aligned, zeroed once
+ *               before its first use (every launch leaves its counters zero).
+ *               One workspace may serve layers of any sizes, one launch after
+ *               another: launches that can overlap (other streams, graphs)
+ *               need their own.  After a launch that gave up a bounded wait
+ *               (spmm24_device_status), zero it again.
+ * flags: SPMM24_BF16, SPMM24_MOE_INT8; SPMM24_STATIC_WEIGHTS and SPMM24_NO_PDL
+ * are accepted and change nothing (the kernel is launched cooperatively, in
+ * stream order).  Allocates nothing.  Asynchronous on `stream`. */
+enum { SPMM24_MOE_INT8 = 32u };
+typedef struct spmm24_moe_layer {
+    int tokens, hidden, inter, experts, top_k;
+    int activation;
+    int norm_topk;
+    const void* x;
+    const void* router;
+    const void* gate_up;
+    const void* gate_up_meta;
+    const void* down;
+    const void* down_meta;
+    const float* gate_up_scale;
+    const float* down_scale;
+    int* topk_ids;
+    float* topk_weights;
+    void* y;
+    const spmm24_epilogue* epilogue;
+    void* workspace;
+    size_t workspace_bytes;
+} spmm24_moe_layer;
+cudaError_t spmm24_launch_moe(cudaStream_t stream, const spmm24_moe_layer* layer, unsigned flags);
+/* 0 for sizes that spmm24_launch_moe does not take. */
+size_t spmm24_moe_workspace_bytes(int tokens, int hidden, int inter, int experts, int top_k, unsigned flags);
+
 /* Packed-weight files (no counterpart in the reference): a 64-byte header
  * (magic "SPMM24W", version 1, dtype 0 = fp16 / 1 = bf16 / 2 = fp8 E4M3 /
  * 3 = fp8 E5M2, M, K, payload sizes, FNV-1a-64 checksum of the payload),
