@@ -1183,10 +1183,11 @@ cudaError_t launch_grouped_impl(cudaStream_t stream, const spmm24_problem* probs
 }
 
 // ------------------------------------------------ mixture-of-experts layer
-// The workspace: counters first, at the same place for every layer's sizes
-// (they are zero between launches, whatever layers share the workspace).
+// The workspace: the counters and the tagged partial tiles first, at the same
+// place for layers of all sizes, so that no launch takes another's values for
+// tags.
 struct MoeLayout {
-    size_t tile_count, logits, xscale, amax, part, xq, h, hq, total;
+    size_t part, logits, xscale, amax, xq, h, hq, total;
     int slots, shares;
 };
 
@@ -1200,17 +1201,15 @@ MoeLayout moe_layout(int T, int H, int I, int E, int k, bool i8) {
         at = (at + bytes + 255) / 256 * 256;
         return here;
     };
-    const int strips = (T + 7) / 8, n_tile = T <= 16 ? 16 : 32;
+    const int strips = (T + 7) / 8;
     l.slots = std::min(E, T * k);
-    // enough K shares of a logit to give every warp of the device one, of at
-    // least 256 inputs (one load of a warp)
-    l.shares = std::max(1, std::min({kMoeMaxCtas * kMoeWarps / (E * strips), (H + 255) / 256, 32}));
+    // K shares of a logit: a load per lane each, while there are CTAs for them
+    l.shares = std::max(1, std::min({128 / (E * strips), (H + 8 * kThreads - 1) / (8 * kThreads), kMoeMaxShares}));
     take(256);
-    l.tile_count = take((size_t)(kMoeMaxTiles + kMoeMaxDownTiles) * 4);
+    l.part = take((size_t)kMoeMaxCtas * 2 * kMoeSlotWords * 8);
     l.logits = take((size_t)l.shares * T * E * 4);
     l.xscale = take(kMoeMaxTokens * 4);
     l.amax = take((size_t)l.slots * kMoeMaxTokens * 4);
-    l.part = take((size_t)kMoeMaxCtas * 2 * kTileM * 2 * n_tile * 4);
     l.xq = take(i8 ? (size_t)T * H : 0);
     l.h = take(i8 ? (size_t)l.slots * T * I * 4 : (size_t)l.slots * strips * I * 16);
     l.hq = take(i8 ? (size_t)l.slots * T * I : 0);
@@ -1249,7 +1248,13 @@ cudaError_t launch_moe_kernel(cudaStream_t stream, int dev, int ctas, const MoeP
     attr[0].val.cooperative = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
+#ifdef SPMM24_TRACE
+    MoeParams mt = mp;
+    mt.trace_base = g_trace_next.fetch_add(ctas);
+    return cudaLaunchKernelEx(&cfg, kern, mt);
+#else
     return cudaLaunchKernelEx(&cfg, kern, mp);
+#endif
 }
 
 cudaError_t launch_moe_impl(cudaStream_t stream, const spmm24_moe_layer* L, unsigned flags) {
@@ -1302,11 +1307,11 @@ cudaError_t launch_moe_impl(cudaStream_t stream, const spmm24_moe_layer* L, unsi
     mp.max_slots = lay.slots;
     mp.logit_shares = lay.shares;
     mp.bar = reinterpret_cast<uint32_t*>(ws);
-    mp.tile_count = reinterpret_cast<uint32_t*>(ws + lay.tile_count);
+    mp.epoch = mp.bar + 32;
     mp.logits = reinterpret_cast<float*>(ws + lay.logits);
     mp.xscale = reinterpret_cast<float*>(ws + lay.xscale);
     mp.amax = reinterpret_cast<uint32_t*>(ws + lay.amax);
-    mp.part = reinterpret_cast<float*>(ws + lay.part);
+    mp.part = reinterpret_cast<uint64_t*>(ws + lay.part);
     mp.xq = reinterpret_cast<int8_t*>(ws + lay.xq);
     mp.h32 = reinterpret_cast<float*>(ws + lay.h);
     mp.h16 = reinterpret_cast<uint16_t*>(ws + lay.h);

@@ -22,10 +22,10 @@
 //     expert; 16 or 32 columns cost the tensor core nothing beside the stream.
 //   - Work is cut into K stages, not tiles: the gate / up phase has (expert,
 //     128 rows, stage) units, the down phase (128 rows, expert, stage) ones,
-//     and every CTA takes an equal run of them, whatever the routing.  Tiles
-//     that several CTAs share are summed by the last of them to finish, from
-//     fp32 partial tiles in the workspace, in the order of the K stages --
-//     the same order whoever is last, so results do not depend on timing.
+//     and every CTA takes an equal run of them, whatever the routing.  A tile
+//     that several CTAs share is finished by the first of them, which adds the
+//     others' fp32 (int8: integer) partials out of the workspace in the order
+//     of the K stages, so results do not depend on timing.
 //   - A grid barrier separates the phases (cooperative launch: all CTAs are
 //     resident).  The producer fills the ring with the down phase's first
 //     weights before it waits there, so the stream goes on over the barrier.
@@ -46,8 +46,8 @@ constexpr int kMoeMaxTokens = 32;
 constexpr int kMoeMaxExperts = 256;
 constexpr int kMoeMaxTopK = 16;
 constexpr int kMoeMaxCtas = 160;
-constexpr int kMoeMaxTiles = 32768;     // (expert, 128 rows of I) tiles of the gate / up phase
-constexpr int kMoeMaxDownTiles = 4096;  // 128-row tiles of H
+constexpr int kMoeMaxTiles = 32768;  // (expert, 128 rows of I) tiles of the gate / up phase
+constexpr int kMoeMaxShares = 4;  // K shares of a logit
 constexpr int kMoeWarps = kThreads / 32;
 
 struct MoeParams {
@@ -68,16 +68,17 @@ struct MoeParams {
     int max_slots;            // min(E, T k): experts that can be in use
     int logit_shares;         // K shares of a logit
     // workspace
-    uint32_t* bar;            // arrivals, generation
-    uint32_t* tile_count;     // gate / up tiles, then down tiles; zero between launches
+    uint32_t* bar;            // arrivals at the grid barrier
+    uint32_t* epoch;          // launches so far: the tags of this launch's partials
     float* logits;            // [share][T][E]
-    float* part;              // [CTA][2][N_TILE / 2 quads][128 rows][4]
+    uint64_t* part;           // [CTA][2][32 column pairs][128 rows][2] {value, tag}
     uint32_t* amax;           // int8: [slot][32] largest |h| (bits)
     float* xscale;            // int8: [32]
     int8_t* xq;               // int8: T x H
     float* h32;               // int8: [slot][T][I]
     int8_t* hq;               // int8: [slot][T][I]
     uint16_t* h16;            // 16-bit: [slot][strips][I][8]
+    SPMM24_TRACE_FIELD
 };
 
 constexpr int moe_stages(int n_tile, bool i8) { return n_tile == 16 ? 9 : i8 ? 7 : 8; }
@@ -103,40 +104,52 @@ struct MoeShared {
     uint16_t list[kMoeMaxExperts];               // experts in use, in increasing order
     float xscale[kMoeMaxTokens];
     uint32_t red[kMoeWarps][8];
-    uint32_t top[8];
-    uint32_t tmem, gen0, n_active, last, dead;
+    uint32_t top[kMoeMaxTokens];
+    uint32_t tmem, base, epoch, n_active, last, dead;
 };
 static_assert(sizeof(MoeShared) <= 6144, "MoeCfg reserves 6 KB");
 
 // ------------------------------------------------------------ grid barrier
-// One arrival per CTA; the last one resets the count and starts the next
-// generation.  gen0 is the generation read before the CTA's first arrival, so
-// the launch's n-th barrier is over once the generation has passed gen0 + n.
+// One word that counts arrivals, `ctas` per barrier, and wraps at a multiple
+// of that (so it stays a multiple between launches).  Before a CTA's own first
+// arrival the launch's first barrier cannot be over, so the word then read,
+// rounded down to a multiple, is the launch's base, and its n-th barrier is
+// over once the count has reached base + n ctas.  One atomic and one poll:
+// 1.5 us, where a count that the last CTA resets before it publishes a
+// generation takes three round trips (2.3 us).
+__device__ __forceinline__ uint32_t moe_wrap(uint32_t ctas) { return ctas << 20; }
 __device__ __forceinline__ void moe_arrive(uint32_t* bar, uint32_t ctas) {
     __threadfence();
-    if (atomicAdd(bar, 1u) == ctas - 1u) {
-        bar[0] = 0u;
-        __threadfence();
-        atomicAdd(bar + 1, 1u);
-    }
+    atomicInc(bar, moe_wrap(ctas) - 1u);
 }
-__device__ __forceinline__ bool moe_wait(const uint32_t* bar, uint32_t gen) {
+__device__ __forceinline__ bool moe_wait(const uint32_t* bar, uint32_t base, uint32_t n, uint32_t ctas) {
+    const uint32_t wrap = moe_wrap(ctas);
+    uint32_t target = base + n * ctas;
+    if (target >= wrap) target -= wrap;
     const uint64_t t0 = ptx::globaltimer();
     uint32_t spins = 0;
-    while ((int)(ptx::ld_acquire_gpu(bar + 1) - gen) < 0) {
+    while (true) {
+        const uint32_t c = ptx::ld_acquire_gpu(bar);
+        if ((c >= target ? c - target : c + wrap - target) < wrap / 2) return true;
         if ((++spins & 255u) == 0u && ptx::globaltimer() - t0 > kWaitLimitNs) {
             atomicOr(&g_spmm24_status, kStatusBarrierTimeout);
             return false;
         }
     }
-    return true;
 }
 
-// An equal run of the units 0 .. U - 1 for each of `ctas` CTAs (ctas <= U).
-__device__ __forceinline__ int moe_begin(int units, int cta, int ctas) { return (int)((long long)units * cta / ctas); }
-__device__ __forceinline__ int moe_owner(int units, int unit, int ctas) {
-    return (int)((((long long)unit + 1) * ctas - 1) / units);
-}
+// An equal run of the units 0 .. U - 1 for each CTA: q or (the first r CTAs)
+// q + 1 of them.
+struct MoeRuns {
+    int units, ctas, q, r;  // ctas <= units
+    __device__ __forceinline__ MoeRuns(int units_, int grid)
+        : units(units_), ctas(min(grid, units_)), q(ctas ? units / ctas : 0), r(units - q * ctas) {}
+    __device__ __forceinline__ int begin(int cta) const { return cta < ctas ? cta * q + min(cta, r) : units; }
+    __device__ __forceinline__ int owner(int unit) const {
+        const int big = r * (q + 1);
+        return unit < big ? unit / (q + 1) : r + (unit - big) / q;
+    }
+};
 
 // SiLU and GELU (tanh form, as y sigmoid(2 z)) to fp32 accuracy: the few
 // values of this layer are no load, and h is rounded after them.
@@ -148,12 +161,14 @@ __device__ __forceinline__ float moe_activate(float y, int act) {
 }
 
 // ------------------------------------------------------------------ router
-// Unit (expert, strip of eight tokens, K share): one warp, eight partial
-// logits.  A lane takes eight consecutive inputs at a time.
+// Unit (expert, strip of eight tokens, K share): a block, eight partial
+// logits.  A lane takes eight consecutive inputs at a time.  Shares of about
+// one load per lane, summed over the block's warps here, leave few values to
+// add per logit after the grid barrier, where latency counts.
 template <bool BF16>
-__device__ __forceinline__ void moe_router(const MoeParams& p, int unit0, int step, int lane) {
-    const int shares = p.logit_shares, groups = p.H / 8, per = (groups + shares - 1) / shares;
-    const int units = p.E * p.strips * shares;
+__device__ __forceinline__ void moe_router(const MoeParams& p, MoeShared& sh, int unit0, int step) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int shares = p.logit_shares, groups = p.H / 8, units = p.E * p.strips * shares;
     for (int it = unit0; it < units; it += step) {
         const int ks = it % shares, s = it / shares % p.strips, e = it / shares / p.strips;
         const uint4* wrow = reinterpret_cast<const uint4*>(p.router + (size_t)e * p.H);
@@ -161,8 +176,8 @@ __device__ __forceinline__ void moe_router(const MoeParams& p, int unit0, int st
         float acc[8];
 #pragma unroll
         for (int t = 0; t < 8; ++t) acc[t] = 0.f;
-        const int g1 = min(groups, (ks + 1) * per);
-        for (int g = ks * per + lane; g < g1; g += 32) {
+        const int g1 = (int)((long long)groups * (ks + 1) / shares);
+        for (int g = (int)((long long)groups * ks / shares) + (int)threadIdx.x; g < g1; g += kThreads) {
             const uint4 w4 = wrow[g];
             uint4 xv[8];
 #pragma unroll
@@ -183,78 +198,82 @@ __device__ __forceinline__ void moe_router(const MoeParams& p, int unit0, int st
                 }
             }
         }
+        // eight sums over 32 lanes, halving the values with the lanes: the
+        // lane ends with the sum of token 4 (lane / 16) + 2 (lane / 8 % 2) + lane / 4 % 2
 #pragma unroll
-        for (int t = 0; t < 8; ++t)
+        for (int n = 4, o = 16; n; n >>= 1, o >>= 1) {
 #pragma unroll
-            for (int o = 16; o; o >>= 1) acc[t] += __shfl_xor_sync(0xffffffffu, acc[t], o);
-#pragma unroll
-        for (int t = 0; t < 8; ++t)
-            if (lane == t && 8 * s + t < p.T) p.logits[((size_t)ks * p.T + 8 * s + t) * p.E + e] = acc[t];
+            for (int t = 0; t < n; ++t) {
+                const float give = lane & o ? acc[t] : acc[t + n], keep = lane & o ? acc[t + n] : acc[t];
+                acc[t] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+            }
+        }
+        acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], 2);
+        acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], 1);
+        if ((lane & 3) == 0) sh.red[warp][lane >> 2] = __float_as_uint(acc[0]);
+        __syncthreads();
+        const int t = 8 * s + (int)threadIdx.x;
+        if (threadIdx.x < 8 && t < p.T) {
+            float l = 0.f;
+            for (int w = 0; w < kMoeWarps; ++w) l += __uint_as_float(sh.red[w][threadIdx.x]);
+            p.logits[((size_t)ks * p.T + t) * p.E + e] = l;
+        }
+        __syncthreads();  // sh.red is free again
     }
 }
 
-// Top k of one token's logits and their weights; one warp.  Keys order as the
-// logits do, NaN above all (it then makes every weight NaN).
-__device__ __forceinline__ void moe_top_k(const MoeParams& p, MoeShared& sh, int t, int lane, bool publish) {
-    float l[kMoeMaxExperts / 32];
-    uint32_t key[kMoeMaxExperts / 32];
-#pragma unroll
-    for (int i = 0; i < kMoeMaxExperts / 32; ++i) {
-        const int e = lane + 32 * i;
-        l[i] = 0.f;
-        key[i] = 0u;
-        if (e < p.E) {
-            float v = 0.f;
-            for (int s = 0; s < p.logit_shares; ++s) v += __ldcg(p.logits + ((size_t)s * p.T + t) * p.E + e);
-            l[i] = v;
-            const uint32_t b = __float_as_uint(v + 0.f);  // -0 -> +0: the two are a tie
-            key[i] = v != v ? 0xffffffffu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
+// A logit's key: keys order as the logits do, NaN above all (it then makes
+// every weight of its token NaN); -0 and +0 are a tie.
+__device__ __forceinline__ uint32_t moe_key(float v) {
+    const uint32_t b = __float_as_uint(v + 0.f);
+    return v != v ? 0xffffffffu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+
+// Top k of every token, by rank: an expert's place is the number of its
+// token's experts that come before it, and those of the first k places write
+// themselves down.  A thread per (token, expert), each against all: choosing
+// one after another is a chain of warp reductions (T = 8, E = 64, k = 8: 6.6 us
+// against 1 for this).  l, key: [T][pitch] logits and keys in shared memory,
+// padded with keys 0; l is left holding exp(l - largest).  All threads.
+__device__ __forceinline__ void moe_top_k(const MoeParams& p, MoeShared& sh, float* l, const uint32_t* key, int pitch,
+                                          bool publish) {
+    const int n = p.T * p.E;
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        const int t = i / p.E, e = i - t * p.E;
+        const uint4* row = reinterpret_cast<const uint4*>(key + t * pitch);
+        const uint32_t mine = key[t * pitch + e];
+        int place = 0;
+#pragma unroll 2
+        for (int g = 0; g < pitch / 4; ++g) {
+            const uint4 v = row[g];
+            place += (v.x > mine || (v.x == mine && 4 * g < e)) + (v.y > mine || (v.y == mine && 4 * g + 1 < e)) +
+                     (v.z > mine || (v.z == mine && 4 * g + 2 < e)) + (v.w > mine || (v.w == mine && 4 * g + 3 < e));
+        }
+        if (place < p.k) {
+            sh.ids[t * p.k + place] = e;
+            if (place == 0) sh.top[t] = __float_as_uint(l[t * pitch + e]);
+            atomicOr(&sh.mask[e], 1u << t);
         }
     }
-    int my_id = -1;
-    float my_l = 0.f;
-    for (int j = 0; j < p.k; ++j) {
-        uint32_t best = 0u;
-        int bi = 0;
-        float bl = 0.f;
-#pragma unroll
-        for (int i = 0; i < kMoeMaxExperts / 32; ++i)
-            if (key[i] > best) {
-                best = key[i];
-                bi = i;
-                bl = l[i];
-            }
-        const uint32_t m = __reduce_max_sync(0xffffffffu, best);
-        const uint32_t win = __reduce_min_sync(0xffffffffu, best == m ? (uint32_t)(lane + 32 * bi) : 0xffffffffu);
-        const float lw = __shfl_sync(0xffffffffu, bl, (int)(win & 31u));
-        if (lane == (int)(win & 31u)) {
-#pragma unroll
-            for (int i = 0; i < kMoeMaxExperts / 32; ++i)
-                if (i == (int)(win >> 5)) key[i] = 0u;
-        }
-        if (lane == j) {
-            my_id = (int)win;
-            my_l = lw;
-        }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        const int t = i / p.E, at = t * pitch + i - t * p.E;
+        l[at] = expf(l[at] - __uint_as_float(sh.top[t]));
     }
-    const float top = __shfl_sync(0xffffffffu, my_l, 0);
-    float sum = 0.f;
-    if (p.norm) {
-        sum = lane < p.k ? expf(my_l - top) : 0.f;
-    } else {
-#pragma unroll
-        for (int i = 0; i < kMoeMaxExperts / 32; ++i)
-            if (lane + 32 * i < p.E) sum += expf(l[i] - top);
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane < p.k) {
-        const float w = expf(my_l - top) / sum;
-        sh.ids[t * p.k + lane] = my_id;
-        sh.weights[t * p.k + lane] = w;
+    __syncthreads();
+    for (int i = threadIdx.x; i < p.T * p.k; i += kThreads) {
+        const int t = i / p.k;
+        const float* lt = l + t * pitch;
+        float sum = 0.f;
+        if (p.norm)
+            for (int j = 0; j < p.k; ++j) sum += lt[sh.ids[t * p.k + j]];
+        else
+            for (int e = 0; e < p.E; ++e) sum += lt[e];
+        const float w = lt[sh.ids[i]] / sum;
+        sh.weights[i] = w;
         if (publish) {
-            if (p.ids) p.ids[t * p.k + lane] = my_id;
-            if (p.weights) p.weights[t * p.k + lane] = w;
+            if (p.ids) p.ids[i] = sh.ids[i];
+            if (p.weights) p.weights[i] = w;
         }
     }
 }
@@ -268,13 +287,18 @@ __device__ __forceinline__ void moe_quantize_x(const MoeParams& p, MoeShared& sh
     const uint4* strip = reinterpret_cast<const uint4*>(p.x) + (size_t)s * p.H;
     const uint32_t abs2 = 0x7fff7fffu;
     uint32_t m[4] = {0u, 0u, 0u, 0u};
-#pragma unroll 4
-    for (int c = threadIdx.x; c < p.H; c += kThreads) {
-        const uint4 v = strip[c];
-        m[0] = vmaxu2(m[0], v.x & abs2);
-        m[1] = vmaxu2(m[1], v.y & abs2);
-        m[2] = vmaxu2(m[2], v.z & abs2);
-        m[3] = vmaxu2(m[3], v.w & abs2);
+    for (int c0 = threadIdx.x; c0 < p.H; c0 += 12 * kThreads) {
+        uint4 v[12];  // twelve loads in flight
+#pragma unroll
+        for (int i = 0; i < 12; ++i)
+            v[i] = c0 + i * kThreads < p.H ? strip[c0 + i * kThreads] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int i = 0; i < 12; ++i) {
+            m[0] = vmaxu2(m[0], v[i].x & abs2);
+            m[1] = vmaxu2(m[1], v[i].y & abs2);
+            m[2] = vmaxu2(m[2], v[i].z & abs2);
+            m[3] = vmaxu2(m[3], v[i].w & abs2);
+        }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -366,54 +390,84 @@ __device__ __forceinline__ uint32_t moe_add(uint32_t a, uint32_t b) {
     return I8 ? a + b : __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
 }
 
-// A tile that several CTAs share: this CTA's partial (NV words per row, the
-// first 4 tq of every N_TILE of them in use) goes to the workspace; the last
-// CTA to get here adds all partials in K order into v and returns true.
-// INT: the words are 32-bit integers.  Called by the 128 epilogue threads.
-template <int N_TILE, int NV, bool INT>
-__device__ __forceinline__ bool moe_share_tile(const MoeParams& p, MoeShared& sh, uint32_t (&v)[NV], int row, int units,
-                                               int ctas, int tile, int stages, uint32_t* count) {
-    constexpr int SLOT = kTileM * 2 * N_TILE;  // floats of one partial
-    const int tq = (p.T + 3) / 4, first = tile * stages;
-    const int c0 = moe_owner(units, first, ctas), c1 = moe_owner(units, first + stages - 1, ctas);
-    const int me = (int)blockIdx.x;
-    // A CTA's run touches a shared tile with its first segment (slot 0) or its last (slot 1).
-    auto base = [&](int c) {
-        return reinterpret_cast<uint4*>(p.part + ((size_t)c * 2 + (moe_begin(units, c, ctas) < first ? 1 : 0)) * SLOT) + row;
-    };
-    uint4* own = base(me);
-#pragma unroll
-    for (int q = 0; q < NV / 4; ++q)
-        if (q % (N_TILE / 4) < tq)
-            __stcg(own + (size_t)q * kTileM, make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]));
-    __threadfence();
-    ptx::named_barrier(kBarEpi, kEpiThreads);
-    if (threadIdx.x == 64) {
-        const bool last = atomicAdd(count + tile, 1u) == (uint32_t)(c1 - c0);
-        if (last) count[tile] = 0u;  // for the next launch
-        sh.last = last ? 1u : 0u;
-        __threadfence();
+// Two 64-bit words {value, tag, value, tag}: each word is read as it was
+// written, so a word with the right tag holds its value -- the partial needs no
+// fence, flag or counter (with those, a shared tile cost 5 us; so 2).
+__device__ __forceinline__ void moe_put2(uint64_t* p, uint32_t a, uint32_t b, uint32_t tag) {
+    asm volatile("st.relaxed.gpu.global.v2.b64 [%0], {%1, %2};" ::"l"(p), "l"((uint64_t)tag << 32 | a),
+                 "l"((uint64_t)tag << 32 | b)
+                 : "memory");
+}
+__device__ __forceinline__ void moe_get2(const uint64_t* p, uint64_t& a, uint64_t& b) {
+    asm volatile("ld.relaxed.gpu.global.v2.b64 {%0, %1}, [%2];" : "=l"(a), "=l"(b) : "l"(p) : "memory");
+}
+
+// A tile that several CTAs share: every one of them writes its partial (the
+// first T columns of every N_TILE of its NV, 32-bit words), and at the end of
+// the phase, when all have written at about the same time, finishes an equal
+// part of the tile's rows from all partials, added in K order.
+struct MoeTile {
+    int first, c0, c1;  // the tile's first unit; the CTAs that share it
+    __device__ __forceinline__ MoeTile(const MoeRuns& runs, int tile, int stages)
+        : first(tile * stages), c0(runs.owner(first)), c1(runs.owner(first + stages - 1)) {}
+    // A CTA's run meets a shared tile at its begin (its slot 0) or, the first
+    // CTA's where the tile is not the first of its run, at its end (slot 1).
+    __device__ __forceinline__ int slot(const MoeRuns& runs, int c) const {
+        return 2 * c + (c == c0 && runs.begin(c) < first ? 1 : 0);
     }
-    ptx::named_barrier(kBarEpi, kEpiThreads);
-    const bool last = sh.last != 0u;
-    ptx::named_barrier(kBarEpi, kEpiThreads);  // sh.last may be written again
-    if (!last) return false;
-    __threadfence();
+};
+constexpr size_t kMoeSlotWords = (size_t)kTileM * 2 * kMoeMaxTokens;
+
+template <int N_TILE, int NV>
+__device__ __forceinline__ void moe_put_partial(const MoeParams& p, const uint32_t (&v)[NV], int row, size_t slot,
+                                                uint32_t tag) {
+    uint64_t* at = p.part + slot * kMoeSlotWords + (size_t)row * 2;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) v[i] = 0u;
-    for (int c = c0; c <= c1; ++c) {
-        const uint4* b = base(c);
+    for (int i = 0; i < NV; i += 2)
+        if (i % N_TILE < p.T) moe_put2(at + (size_t)i * kTileM, v[i], v[i + 1], tag);
+}
+
+// Sums NP column pairs (the words of columns col[n], col[n] + 1) of one row
+// over the tile's CTAs, BATCH of them in flight at once.
+template <int NP, int BATCH, bool INT>
+__device__ __forceinline__ void moe_sum_partials(const MoeParams& p, const MoeRuns& runs, const MoeTile& tile,
+                                                 const int (&col)[NP], int row, uint32_t tag, uint32_t (&sum)[2 * NP], bool& ok) {
 #pragma unroll
-        for (int q = 0; q < NV / 4; ++q)
-            if (q % (N_TILE / 4) < tq) {
-                const uint4 x = __ldcg(b + (size_t)q * kTileM);
-                v[4 * q] = moe_add<INT>(v[4 * q], x.x);
-                v[4 * q + 1] = moe_add<INT>(v[4 * q + 1], x.y);
-                v[4 * q + 2] = moe_add<INT>(v[4 * q + 2], x.z);
-                v[4 * q + 3] = moe_add<INT>(v[4 * q + 3], x.w);
+    for (int n = 0; n < 2 * NP; ++n) sum[n] = 0u;
+    uint64_t t0 = 0;
+#pragma unroll 1
+    for (int c = tile.c0; c <= tile.c1; c += BATCH) {
+        uint64_t x[BATCH][2 * NP];
+        for (uint32_t polls = 1;; ++polls) {
+            bool there = true;
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+                const uint64_t* at = p.part + (size_t)tile.slot(runs, min(c + i, tile.c1)) * kMoeSlotWords + (size_t)row * 2;
+#pragma unroll
+                for (int n = 0; n < NP; ++n) moe_get2(at + (size_t)col[n] * kTileM, x[i][2 * n], x[i][2 * n + 1]);
+            }
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i)
+#pragma unroll
+                for (int n = 0; n < 2 * NP; ++n) there = there && (uint32_t)(x[i][n] >> 32) == tag;
+            if (there || !ok) break;
+            if ((polls & 255u) == 0u) {
+                const uint64_t now = ptx::globaltimer();
+                if (!t0) t0 = now;
+                if (now - t0 > kWaitLimitNs) {
+                    atomicOr(&g_spmm24_status, kStatusEpilogueTimeout);
+                    ok = false;
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i)
+            if (c + i <= tile.c1) {
+#pragma unroll
+                for (int n = 0; n < 2 * NP; ++n) sum[n] = moe_add<INT>(sum[n], (uint32_t)x[i][n]);
             }
     }
-    return true;
+    ok = __all_sync(0xffffffffu, ok);
 }
 
 template <int N_TILE, bool I8>
@@ -432,6 +486,7 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
     const int cta = (int)blockIdx.x, grid = (int)gridDim.x;
 
     if (threadIdx.x == 0) {
+        SPMM24_STAMP(0);
         for (int s = 0; s < STAGES; ++s) {
             ptx::mbar_init(&full[s], 1);
             ptx::mbar_init(&empty[s], 1);
@@ -441,7 +496,9 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
             ptx::mbar_init(&acc_empty[b], kEpiThreads / 32);
         }
         ptx::fence_mbarrier_init();
-        sh.gen0 = ptx::ld_acquire_gpu(p.bar + 1);  // before this CTA's first arrival
+        const uint32_t c = ptx::ld_acquire_gpu(p.bar);  // before this CTA's first arrival
+        sh.base = c - c % (uint32_t)grid;
+        sh.epoch = ptx::ld_acquire_gpu(p.epoch);
         sh.dead = 0u;
         ptx::prefetch_tmap(&p.tmGU);
         ptx::prefetch_tmap(&p.tmGUE);
@@ -456,9 +513,6 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
     }
     for (int e = threadIdx.x; e < kMoeMaxExperts; e += kThreads) sh.mask[e] = 0u;
     ptx::tc_fence_before();
-    __syncthreads();
-    ptx::tc_fence_after();
-    const uint32_t tmem_base = sh.tmem;
 
     // ------------------------------------------- router, rounding of x
     int quant_ctas = 0;
@@ -474,37 +528,60 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
     }
     if (p.router) {
         // the CTAs that do not round x come first
-        const int unit0 = ((cta + grid - quant_ctas % grid) % grid) * kMoeWarps + warp;
-        if (p.bf16) moe_router<true>(p, unit0, grid * kMoeWarps, lane);
-        else moe_router<false>(p, unit0, grid * kMoeWarps, lane);
+        const int unit0 = (cta + grid - quant_ctas % grid) % grid;
+        if (p.bf16) moe_router<true>(p, sh, unit0, grid);
+        else moe_router<false>(p, sh, unit0, grid);
     }
-    uint32_t gen = sh.gen0;
+    if constexpr (I8) ptx::fence_proxy_async_global();  // xq is read by TMA
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem_base = sh.tmem;
+    const uint32_t base = sh.base, tag = 2u * sh.epoch + 1u;  // zeroed memory holds no tag
+    uint32_t barriers = 0;  // of this launch, so far
     if (I8 || p.router) {
-        if constexpr (I8) ptx::fence_proxy_async_global();  // xq is read by TMA
-        __syncthreads();
-        ++gen;
+        ++barriers;
         if (threadIdx.x == 0) {
             moe_arrive(p.bar, (uint32_t)grid);
-            if (!moe_wait(p.bar, gen)) sh.dead = 1u;
+            if (!moe_wait(p.bar, base, barriers, (uint32_t)grid)) sh.dead = 1u;
             __threadfence();
         }
         __syncthreads();
     }
 
     // --------------------------------------------------------- routing
+    if (I8 && threadIdx.x < p.T) sh.xscale[threadIdx.x] = __ldcg(p.xscale + threadIdx.x);
     if (p.router) {
-        for (int t = warp; t < p.T; t += kMoeWarps) moe_top_k(p, sh, t, lane, cta == 0);
+        // T x E logits and keys in the ring, which is still idle
+        const int pitch = (p.E + 3) / 4 * 4, n = p.T * pitch, logits = p.T * p.E;
+        uint32_t* key = reinterpret_cast<uint32_t*>(smem);
+        float* l = reinterpret_cast<float*>(key + n);
+#pragma unroll 2
+        for (int i = threadIdx.x; i < n; i += kThreads) {
+            const int t = i / pitch, e = i - t * pitch;
+            const float* at = p.logits + t * p.E + e;
+            float v[kMoeMaxShares];
+#pragma unroll
+            for (int s = 0; s < kMoeMaxShares; ++s)
+                v[s] = e < p.E && s < p.logit_shares ? __ldcg(at + (size_t)s * logits) : 0.f;
+            float sum = v[0];
+#pragma unroll
+            for (int s = 1; s < kMoeMaxShares; ++s)
+                if (s < p.logit_shares) sum += v[s];
+            key[i] = e < p.E ? moe_key(sum) : 0u;
+            l[i] = sum;
+        }
+        __syncthreads();
+        moe_top_k(p, sh, l, key, pitch, cta == 0);
+        ptx::fence_proxy_async_smem();  // before TMA writes the ring
     } else {
         for (int i = threadIdx.x; i < p.T * p.k; i += kThreads) {
             const int e = p.ids[i];
-            sh.ids[i] = e >= 0 && e < p.E ? e : -1;
+            const bool some = e >= 0 && e < p.E;
+            sh.ids[i] = some ? e : -1;
             sh.weights[i] = p.weights[i];
+            if (some) atomicOr(&sh.mask[e], 1u << (i / p.k));
         }
     }
-    if (I8 && threadIdx.x < p.T) sh.xscale[threadIdx.x] = __ldcg(p.xscale + threadIdx.x);
-    __syncthreads();
-    for (int i = threadIdx.x; i < p.T * p.k; i += kThreads)
-        if (sh.ids[i] >= 0) atomicOr(&sh.mask[sh.ids[i]], 1u << (i / p.k));
     __syncthreads();
     if (warp == 0) {
         int n = 0;
@@ -518,6 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
     }
     __syncthreads();
 
+    if (threadIdx.x == 0) SPMM24_STAMP(3);
     const int n_active = sh.dead ? 0 : (int)sh.n_active;
     const int stage_k = I8 ? 256 : 128;
     const int gu_groups = p.H * 2 / stage_k, d_groups = p.I * 2 / stage_k;  // metadata groups along K
@@ -525,10 +603,9 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
     const int i_tiles = (p.I + kTileM - 1) / kTileM, h_tiles = (p.H + kTileM - 1) / kTileM;
     // gate / up: unit (slot, 128 rows of I, stage); down: unit (128 rows of H, slot, stage)
     const int U1 = n_active * i_tiles * S1, S2 = n_active * Se, U2 = h_tiles * S2;
-    const int G1 = min(grid, U1), G2 = min(grid, U2);
-    const int b1 = cta < G1 ? moe_begin(U1, cta, G1) : 0, e1 = cta < G1 ? moe_begin(U1, cta + 1, G1) : 0;
-    const int b2 = cta < G2 ? moe_begin(U2, cta, G2) : 0, e2 = cta < G2 ? moe_begin(U2, cta + 1, G2) : 0;
-    const uint32_t gen_h = gen + (I8 ? 2u : 1u);  // h (int8: rounded) is complete
+    const MoeRuns runs1(U1, grid), runs2(U2, grid);
+    const int b1 = runs1.begin(cta), e1 = runs1.begin(cta + 1), b2 = runs2.begin(cta), e2 = runs2.begin(cta + 1);
+    const uint32_t bar_h = barriers + (I8 ? 2u : 1u);  // h (int8: rounded) is complete
 
     if (warp == 0) {
         // ------------------------------------------------ TMA producer
@@ -582,7 +659,8 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
                 }
             }
             if (ok && b2 < e2) {
-                ok = moe_wait(p.bar, gen_h);
+                ok = moe_wait(p.bar, base, bar_h, (uint32_t)grid);
+                SPMM24_STAMP(5);
                 ptx::fence_proxy_async_global();
                 if (ok) {
                     for (int i = 0; i < ahead; ++i) acts2(b2 + i, it + i);
@@ -636,6 +714,7 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
             for (int s = s0; s < s1 && ok; ++s, it += 2) {
                 for (int half = 0; half < 2; ++half) {
                     if (!(ok = wait_full(it + half))) break;
+                    if (lane == 0 && it + half == 0) SPMM24_STAMP(1);
                     if (2 * s + 1 >= gu_groups)
                         patch_tail_metadata<C_>(smem + (it + half) % STAGES * C_::STAGE_BYTES, lane);
                     if (lane == 0) {
@@ -654,6 +733,7 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
             ++j;
             u += s1 - s0;
         }
+        if (lane == 0) SPMM24_STAMP(2);
         for (int u = b2; u < e2 && ok;) {  // a segment ends with its expert: the epilogue weighs each on its own
             const int s0 = u % Se, s1 = min(Se, s0 + e2 - u);
             if (!(ok = begin_acc())) break;
@@ -673,6 +753,7 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
             ++j;
             u += s1 - s0;
         }
+        if (lane == 0) SPMM24_STAMP(7);
     } else {
         // ---------------------------------------------------- epilogue
         const int quad = warp & 3, row = quad * 32 + lane;  // thread = output row (TMEM lane)
@@ -703,9 +784,10 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
             moe_read_acc<2 * N_TILE>(tmem_row + (uint32_t)((j & 1) * 2 * N_TILE), v);
             ptx::tmem_wait_ld();
             release_acc();
-            if (s1 - s0 < S1 &&
-                !moe_share_tile<N_TILE, 2 * N_TILE, I8>(p, sh, v, row, U1, G1, tile, S1, p.tile_count))
+            if (s1 - s0 < S1) {
+                moe_put_partial<N_TILE>(p, v, row, (size_t)cta * 2 + (b1 < tile * S1 ? 1 : 0), tag);
                 continue;
+            }
             const int slot = tile / i_tiles, e = sh.list[slot], r = tile % i_tiles * kTileM + row;
             const bool live = r < p.I;
             if constexpr (I8) {
@@ -741,6 +823,76 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
                 }
             }
         }
+        // The tiles that this CTA shares, first and last of its run.  A warp
+        // takes 32 rows and one or two pairs of tokens at a time.
+        constexpr int PAIRS = N_TILE / 16, BATCH = N_TILE == 16 ? 8 : 4;
+        auto shared_tiles = [&](int b, int e, int stages, const MoeRuns& runs, auto&& f) {
+            if (b >= e) return;
+            const int t0 = b / stages, t1 = (e - 1) / stages;
+            for (int t = t0; t <= t1; t += max(1, t1 - t0)) {
+                if (max(b, t * stages) == t * stages && min(e, (t + 1) * stages) == (t + 1) * stages) continue;
+                const MoeTile tile(runs, t, stages);
+                const int n = tile.c1 - tile.c0 + 1, i = cta - tile.c0;
+                f(t, tile, kTileM * i / n, kTileM * (i + 1) / n);
+            }
+        };
+        shared_tiles(b1, e1, S1, runs1, [&](int t, const MoeTile& tile, int r0, int r1) {
+            const int slot = t / i_tiles, e = sh.list[slot], blocks = (r1 - r0 + 31) / 32;
+            const int units = blocks * ((p.T + 2 * PAIRS - 1) / (2 * PAIRS));
+            const uint32_t mask = sh.mask[e];
+            for (int w = warp - 2; w < units; w += kEpiThreads / 32) {
+                const int rt = r0 + w % blocks * 32 + lane, t0 = w / blocks * 2 * PAIRS;  // row of the tile, first token
+                const int r = t % i_tiles * kTileM + rt;
+                const bool live = rt < r1 && r < p.I;
+                int col[2 * PAIRS];
+#pragma unroll
+                for (int n = 0; n < PAIRS; ++n) {
+                    // past the last token: its own columns again
+                    const int c = t0 + 2 * n < p.T ? t0 + 2 * n : t0;
+                    col[n] = c;
+                    col[PAIRS + n] = N_TILE + c;
+                }
+                uint32_t v[4 * PAIRS];  // gate values, up values
+                moe_sum_partials<2 * PAIRS, BATCH, I8>(p, runs1, tile, col, min(rt, kTileM - 1), tag, v, ok);
+                float gs = 0.f, us = 0.f;
+                if constexpr (I8) {
+                    if (live) {
+                        gs = p.gu_scale[(size_t)e * 2 * p.I + r];
+                        us = p.gu_scale[(size_t)e * 2 * p.I + p.I + r];
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < PAIRS; ++n) {
+                    if (t0 + 2 * n >= p.T) break;
+                    float h[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int tok = t0 + 2 * n + i;
+                        const uint32_t g = v[2 * n + i], u = v[2 * PAIRS + 2 * n + i];
+                        if constexpr (I8) {
+                            h[i] = 0.f;
+                            if (!(mask >> tok & 1u)) continue;
+                            const float xs = sh.xscale[tok];
+                            if (live) {
+                                h[i] = moe_activate(int8_value((int)g, gs, xs), p.act) * int8_value((int)u, us, xs);
+                                __stcg(p.h32 + ((size_t)slot * p.T + tok) * p.I + r, h[i]);
+                            }
+                            const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(h[i]) & 0x7fffffffu);
+                            if (lane == 0) atomicMax(p.amax + slot * kMoeMaxTokens + tok, m);
+                        } else {
+                            h[i] = moe_activate(__uint_as_float(g), p.act) * __uint_as_float(u);
+                        }
+                    }
+                    if constexpr (!I8) {
+                        const int tok = t0 + 2 * n;
+                        if (live)
+                            *reinterpret_cast<uint32_t*>(p.h16 + (((size_t)slot * p.strips + tok / 8) * p.I + r) * 8 +
+                                                         tok % 8) = pack2(h[0], h[1], p.bf16);
+                    }
+                }
+            }
+        });
+        if (threadIdx.x == 64) SPMM24_STAMP(4);
         // h is in place: this CTA's share
         if (n_active > 0) {
             if constexpr (!I8) ptx::fence_proxy_async_global();  // h is read by TMA
@@ -751,7 +903,7 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
         if constexpr (I8) {
             if (n_active > 0) {
                 // round h: (slot, token) rows in pieces of 512 values, a block each
-                if (threadIdx.x == 64) sh.last = ok && moe_wait(p.bar, gen + 1u) ? 1u : 0u;
+                if (threadIdx.x == 64) sh.last = ok && moe_wait(p.bar, base, barriers + 1u, (uint32_t)grid) ? 1u : 0u;
                 ptx::named_barrier(kBarEpi, kEpiThreads);
                 ok = ok && sh.last != 0u;
                 ptx::named_barrier(kBarEpi, kEpiThreads);
@@ -828,11 +980,37 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
                 s = min(s1, (slot + 1) * Se);
             }
             u += s1 - s0;
-            if (s1 - s0 < S2 &&
-                !moe_share_tile<N_TILE, N_TILE, false>(p, sh, y, row, U2, G2, tile, S2, p.tile_count + kMoeMaxTiles))
-                continue;
-            finish(y, tile);
+            if (s1 - s0 < S2)
+                moe_put_partial<N_TILE>(p, y, row, (size_t)cta * 2 + (b2 < tile * S2 ? 1 : 0), tag + 1u);
+            else
+                finish(y, tile);
         }
+        shared_tiles(b2, e2, S2, runs2, [&](int t, const MoeTile& tile, int r0, int r1) {
+            const int cols = p.epi.packed ? 8 * p.strips : p.T, blocks = (r1 - r0 + 31) / 32;
+            const int units = blocks * ((cols + 2 * PAIRS - 1) / (2 * PAIRS));
+            for (int w = warp - 2; w < units; w += kEpiThreads / 32) {
+                const int rt = r0 + w % blocks * 32 + lane, t0 = w / blocks * 2 * PAIRS, gm = t * kTileM + rt;
+                int col[PAIRS];
+#pragma unroll
+                for (int n = 0; n < PAIRS; ++n) col[n] = t0 + 2 * n < p.T ? t0 + 2 * n : 0;
+                uint32_t v[2 * PAIRS];
+                moe_sum_partials<PAIRS, BATCH, false>(p, runs2, tile, col, min(rt, kTileM - 1), tag + 1u, v, ok);
+                if (rt >= r1 || gm >= p.H) continue;
+#pragma unroll
+                for (int i = 0; i < 2 * PAIRS; ++i) {
+                    const int tok = t0 + i;
+                    if (tok >= cols) break;
+                    const size_t at = c_offset(p.epi, gm, tok, p.H, p.T);
+                    float y[1] = {__uint_as_float(v[i])};
+                    if (!plain) {
+                        epilogue_pre<1>(y, p.epi, gm);
+                        if (p.epi.residual && tok < p.T) y[0] += elem_to_f32(p.epi.residual[at], p.epi.bf16);
+                    }
+                    p.y[at] = tok < p.T ? f32_to_elem(y[0], p.epi.bf16) : (uint16_t)0;
+                }
+            }
+        });
+        if (threadIdx.x == 64) SPMM24_STAMP(6);
         if (n_active == 0 && !sh.dead) {  // no token has an expert
             uint32_t y[N_TILE];
 #pragma unroll
@@ -843,6 +1021,8 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
 
     ptx::tc_fence_before();
     __syncthreads();
+    // every CTA that shares a tile has read the epoch before the grid barrier
+    if (cta == 0 && threadIdx.x == 0) *p.epoch = sh.epoch + 1u;
     if (warp == 1) {
         ptx::tc_fence_after();
         ptx::tmem_dealloc(tmem_base, C_::TMEM_COLS);

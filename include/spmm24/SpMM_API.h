@@ -453,7 +453,7 @@ cudaError_t spmm24_launch_int8(cudaStream_t stream, const void* values, const vo
  *   y           H x T 16-bit (with an epilogue that says so, packed B);
  *               epilogue as for spmm24_launch_fused with M = H, N = T, or NULL
  *   workspace   spmm24_moe_workspace_bytes bytes, 256-byte aligned, zeroed once
- *               before its first use (every launch leaves its counters zero).
+ *               before its first use.
  *               One workspace may serve layers of any sizes, one launch after
  *               another: launches that can overlap (other streams, graphs)
  *               need their own.  After a launch that gave up a bounded wait

@@ -395,16 +395,16 @@ def test_other_stream_and_graph(cuda_device):
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph, stream=s):
             _, ids, w = L.run(xs[0], k, ws, y=y, x_packed=xp, stream=s)
-        runs.append((graph, s, xp, y, ids))
+        runs.append((graph, s, xp, y, ids, ws))  # a graph's workspace lives as long as the graph
     torch.cuda.synchronize()
     for i, x in enumerate(xs):
-        for graph, s, xp, y, ids in runs:
+        for graph, s, xp, y, ids, _ in runs:
             with torch.cuda.stream(s):
                 xp.copy_(_strips(x))
                 for _ in range(5):
                     graph.replay()
         torch.cuda.synchronize()
-        for graph, s, xp, y, ids in runs:
+        for graph, s, xp, y, ids, _ in runs:
             assert torch.equal(y[:-64], want[i][0][:-64]) and torch.equal(ids, want[i][1])
     assert spmm24.device_status(0) == 0
 
