@@ -115,6 +115,9 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* m, uin
         : "memory");
 }
 
+// A line into L2 only.
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
 // 16-byte asynchronous global -> shared copy (LDGSTS), grouped and waited
 // for with cp.async.commit_group / wait_group.
 __device__ __forceinline__ void cp_async16(void* dst_smem, const void* src) {

@@ -1206,7 +1206,7 @@ MoeLayout moe_layout(int T, int H, int I, int E, int k, bool i8) {
     // K shares of a logit: a load per lane each, while there are CTAs for them
     l.shares = std::max(1, std::min({128 / (E * strips), (H + 8 * kThreads - 1) / (8 * kThreads), kMoeMaxShares}));
     take(256);
-    l.part = take((size_t)kMoeMaxCtas * 2 * kMoeSlotWords * 8);
+    l.part = take(kMoePartWords * 8);
     l.logits = take((size_t)l.shares * T * E * 4);
     l.xscale = take(kMoeMaxTokens * 4);
     l.amax = take((size_t)l.slots * kMoeMaxTokens * 4);

@@ -26,9 +26,12 @@
 //     that several CTAs share is finished by the first of them, which adds the
 //     others' fp32 (int8: integer) partials out of the workspace in the order
 //     of the K stages, so results do not depend on timing.
-//   - A grid barrier separates the phases (cooperative launch: all CTAs are
-//     resident).  The producer fills the ring with the down phase's first
-//     weights before it waits there, so the stream goes on over the barrier.
+//   - h has to be complete (int8: and rounded, which needs each row's largest
+//     value first) before a down product reads it: grid barriers (cooperative
+//     launch: all CTAs are resident).  The stream does not stop for them: the
+//     experts in use go in two groups A and B, gate / up of A, gate / up of B,
+//     down of A, down of B, and a group's barriers pass while the other's
+//     weights stream; the ring is filled ahead of each.
 //   - Routing weights multiply the down products in fp32, expert by expert, as
 //     they leave TMEM; h stays unscaled.
 //
@@ -48,6 +51,7 @@ constexpr int kMoeMaxTopK = 16;
 constexpr int kMoeMaxCtas = 160;
 constexpr int kMoeMaxTiles = 32768;  // (expert, 128 rows of I) tiles of the gate / up phase
 constexpr int kMoeMaxShares = 4;  // K shares of a logit
+constexpr int kMoeSplitUnits = 8;  // gate / up units per CTA from which the experts go in two groups
 constexpr int kMoeWarps = kThreads / 32;
 
 struct MoeParams {
@@ -81,6 +85,7 @@ struct MoeParams {
     SPMM24_TRACE_FIELD
 };
 
+constexpr int kMoeSharedBytes = 6400;
 constexpr int moe_stages(int n_tile, bool i8) { return n_tile == 16 ? 9 : i8 ? 7 : 8; }
 
 template <int N_TILE, bool I8>
@@ -90,7 +95,7 @@ struct MoeCfg : Cfg<N_TILE, moe_stages(N_TILE, I8), 4, I8> {
     static constexpr int BAR_OFFSET = B_::RING_BYTES;
     static constexpr int NUM_BARS = 2 * STAGES + 4;  // full, empty, acc_full[2], acc_empty[2]
     static constexpr int AUX_OFFSET = (BAR_OFFSET + NUM_BARS * 8 + 15) / 16 * 16;
-    static constexpr int SMEM_BYTES = AUX_OFFSET + 6144;
+    static constexpr int SMEM_BYTES = AUX_OFFSET + kMoeSharedBytes;
     static constexpr int SMEM_ALLOC = SMEM_BYTES + 1024;  // slack to align the base to 1024 B
     static_assert(SMEM_ALLOC <= 232448, "shared memory overflow");
     static_assert(B_::STAGE_BYTES % 1024 == 0, "stages must stay 1024-byte aligned");
@@ -102,12 +107,13 @@ struct MoeShared {
     float weights[kMoeMaxTokens * kMoeMaxTopK];
     uint32_t mask[kMoeMaxExperts];               // tokens of each expert
     uint16_t list[kMoeMaxExperts];               // experts in use, in increasing order
+    uint8_t slot[kMoeMaxExperts];                // an expert's place there
     float xscale[kMoeMaxTokens];
     uint32_t red[kMoeWarps][8];
     uint32_t top[kMoeMaxTokens];
     uint32_t tmem, base, epoch, n_active, last, dead;
 };
-static_assert(sizeof(MoeShared) <= 6144, "MoeCfg reserves 6 KB");
+static_assert(sizeof(MoeShared) <= kMoeSharedBytes, "MoeCfg reserves its bytes");
 
 // ------------------------------------------------------------ grid barrier
 // One word that counts arrivals, `ctas` per barrier, and wraps at a multiple
@@ -118,6 +124,8 @@ static_assert(sizeof(MoeShared) <= 6144, "MoeCfg reserves 6 KB");
 // 1.5 us, where a count that the last CTA resets before it publishes a
 // generation takes three round trips (2.3 us).
 __device__ __forceinline__ uint32_t moe_wrap(uint32_t ctas) { return ctas << 20; }
+// One thread, after a barrier of the block's threads: its fence covers their
+// writes.
 __device__ __forceinline__ void moe_arrive(uint32_t* bar, uint32_t ctas) {
     __threadfence();
     atomicInc(bar, moe_wrap(ctas) - 1u);
@@ -416,41 +424,57 @@ struct MoeTile {
         return 2 * c + (c == c0 && runs.begin(c) < first ? 1 : 0);
     }
 };
+// 64-bit words of a gate / up partial (a down partial takes half of them).
 constexpr size_t kMoeSlotWords = (size_t)kTileM * 2 * kMoeMaxTokens;
+// Partials of the first group's down run lie behind those of the others.
+constexpr size_t kMoePartWords = (size_t)kMoeMaxCtas * 3 * kMoeSlotWords;
 
+// pairs: bit n, columns 2n and 2n + 1 of every N_TILE are wanted.
 template <int N_TILE, int NV>
-__device__ __forceinline__ void moe_put_partial(const MoeParams& p, const uint32_t (&v)[NV], int row, size_t slot,
+__device__ __forceinline__ void moe_put_partial(uint64_t* slot, const uint32_t (&v)[NV], int row, uint32_t pairs,
                                                 uint32_t tag) {
-    uint64_t* at = p.part + slot * kMoeSlotWords + (size_t)row * 2;
+    uint64_t* at = slot + (size_t)row * 2;
 #pragma unroll
     for (int i = 0; i < NV; i += 2)
-        if (i % N_TILE < p.T) moe_put2(at + (size_t)i * kTileM, v[i], v[i + 1], tag);
+        if (pairs >> (i % N_TILE / 2) & 1u) moe_put2(at + (size_t)i * kTileM, v[i], v[i + 1], tag);
+}
+// Pairs of tokens with a member in `mask`.
+__device__ __forceinline__ uint32_t moe_pairs(uint32_t mask) {
+    uint32_t m = (mask | mask >> 1) & 0x55555555u;  // bit 2n -> bit n
+    m = (m | m >> 1) & 0x33333333u;
+    m = (m | m >> 2) & 0x0f0f0f0fu;
+    m = (m | m >> 4) & 0x00ff00ffu;
+    return (m | m >> 8) & 0xffffu;
 }
 
 // Sums NP column pairs (the words of columns col[n], col[n] + 1) of one row
-// over the tile's CTAs, BATCH of them in flight at once.
-template <int NP, int BATCH, bool INT>
-__device__ __forceinline__ void moe_sum_partials(const MoeParams& p, const MoeRuns& runs, const MoeTile& tile,
-                                                 const int (&col)[NP], int row, uint32_t tag, uint32_t (&sum)[2 * NP], bool& ok) {
+// over `count` partials, BATCH of them in flight at once; slot(i): the i-th
+// partial's words.
+template <int NP, int BATCH, bool INT, class Slot>
+__device__ __forceinline__ void moe_sum_partials(int count, Slot&& slot, const int (&col)[NP], int row, uint32_t tag,
+                                                 uint32_t (&sum)[2 * NP], bool& ok) {
 #pragma unroll
     for (int n = 0; n < 2 * NP; ++n) sum[n] = 0u;
     uint64_t t0 = 0;
 #pragma unroll 1
-    for (int c = tile.c0; c <= tile.c1; c += BATCH) {
+    for (int c = 0; c < count; c += BATCH) {
         uint64_t x[BATCH][2 * NP];
         for (uint32_t polls = 1;; ++polls) {
             bool there = true;
 #pragma unroll
             for (int i = 0; i < BATCH; ++i) {
-                const uint64_t* at = p.part + (size_t)tile.slot(runs, min(c + i, tile.c1)) * kMoeSlotWords + (size_t)row * 2;
+                if (c + i >= count) break;
+                const uint64_t* at = slot(c + i) + (size_t)row * 2;
 #pragma unroll
                 for (int n = 0; n < NP; ++n) moe_get2(at + (size_t)col[n] * kTileM, x[i][2 * n], x[i][2 * n + 1]);
             }
 #pragma unroll
             for (int i = 0; i < BATCH; ++i)
 #pragma unroll
-                for (int n = 0; n < 2 * NP; ++n) there = there && (uint32_t)(x[i][n] >> 32) == tag;
+                for (int n = 0; n < 2 * NP; ++n)
+                    there = there && (c + i >= count || (uint32_t)(x[i][n] >> 32) == tag);
             if (there || !ok) break;
+            ptx::nanosleep_ns(100);  // polls of every CTA at once would crowd out what they wait for
             if ((polls & 255u) == 0u) {
                 const uint64_t now = ptx::globaltimer();
                 if (!t0) t0 = now;
@@ -462,7 +486,7 @@ __device__ __forceinline__ void moe_sum_partials(const MoeParams& p, const MoeRu
         }
 #pragma unroll
         for (int i = 0; i < BATCH; ++i)
-            if (c + i <= tile.c1) {
+            if (c + i < count) {
 #pragma unroll
                 for (int n = 0; n < 2 * NP; ++n) sum[n] = moe_add<INT>(sum[n], (uint32_t)x[i][n]);
             }
@@ -536,7 +560,7 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
     __syncthreads();
     ptx::tc_fence_after();
     const uint32_t tmem_base = sh.tmem;
-    const uint32_t base = sh.base, tag = 2u * sh.epoch + 1u;  // zeroed memory holds no tag
+    const uint32_t base = sh.base, tag = 4u * sh.epoch + 1u;  // zeroed memory holds no tag
     uint32_t barriers = 0;  // of this launch, so far
     if (I8 || p.router) {
         ++barriers;
@@ -588,7 +612,11 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
         for (int e0 = 0; e0 < p.E; e0 += 32) {
             const bool used = e0 + lane < p.E && sh.mask[e0 + lane] != 0u;
             const uint32_t b = __ballot_sync(0xffffffffu, used);
-            if (used) sh.list[n + __popc(b & ((1u << lane) - 1u))] = (uint16_t)(e0 + lane);
+            if (used) {
+                const int place = n + __popc(b & ((1u << lane) - 1u));
+                sh.list[place] = (uint16_t)(e0 + lane);
+                sh.slot[e0 + lane] = (uint8_t)place;
+            }
             n += __popc(b);
         }
         if (lane == 0) sh.n_active = (uint32_t)n;
@@ -601,11 +629,17 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
     const int gu_groups = p.H * 2 / stage_k, d_groups = p.I * 2 / stage_k;  // metadata groups along K
     const int S1 = (gu_groups + 1) / 2, Se = (d_groups + 1) / 2;            // stages of one gate / up, one down product
     const int i_tiles = (p.I + kTileM - 1) / kTileM, h_tiles = (p.H + kTileM - 1) / kTileM;
-    // gate / up: unit (slot, 128 rows of I, stage); down: unit (128 rows of H, slot, stage)
-    const int U1 = n_active * i_tiles * S1, S2 = n_active * Se, U2 = h_tiles * S2;
-    const MoeRuns runs1(U1, grid), runs2(U2, grid);
-    const int b1 = runs1.begin(cta), e1 = runs1.begin(cta + 1), b2 = runs2.begin(cta), e2 = runs2.begin(cta + 1);
-    const uint32_t bar_h = barriers + (I8 ? 2u : 1u);  // h (int8: rounded) is complete
+    // Two groups of experts (the first nA in use, the others), unless there is
+    // little work: gate / up of A, of B, down of A, of B.
+    const bool split = n_active > 1 && h_tiles <= grid &&
+                       (long long)n_active * i_tiles * S1 >= (long long)kMoeSplitUnits * grid;
+    const int nA = split ? (n_active + 1) / 2 : n_active, n_groups = split ? 2 : 1;
+    // gate / up units (slot, 128 rows of I, stage), down units (128 rows of H, slot, stage) of one group
+    auto first_of = [&](int g) { return g ? nA : 0; };
+    auto count_of = [&](int g) { return g ? n_active - nA : nA; };
+    auto runs1_of = [&](int g) { return MoeRuns(count_of(g) * i_tiles * S1, grid); };
+    auto runs2_of = [&](int g) { return MoeRuns(h_tiles * count_of(g) * Se, grid); };
+    auto h_done = [&](int g) { return barriers + (I8 ? 2u * g + 2u : g + 1u); };  // barrier after a group's h is in place
 
     if (warp == 0) {
         // ------------------------------------------------ TMA producer
@@ -613,8 +647,7 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
             const uint64_t pol_stream = ptx::policy_evict_first(), pol_keep = ptx::policy_evict_last();
             const uint32_t acts_bytes = I8 ? C_::B_BYTES : (uint32_t)p.strips * 2048u;
             const uint32_t w_bytes = C_::A_BYTES + C_::E_BYTES;
-            if constexpr (I8) ptx::fence_proxy_async_global();
-            int it = 0, issued = 0;  // ring slots used by the gate / up phase; armed in all
+            int it = 0, issued = 0;  // ring slots so far; armed in all
             bool ok = true;
             auto slot_of = [&](int i) { return i % STAGES; };
             auto acquire = [&](int i, uint32_t bytes) {
@@ -627,49 +660,75 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
                 issued = i + 1;
                 return true;
             };
-            for (int u = b1; u < e1 && ok; ++u) {
-                const int tile = u / S1, s = u % S1;
-                const int e = sh.list[tile / i_tiles], row0 = e * 2 * p.I + tile % i_tiles * kTileM;
-                for (int half = 0; half < 2 && ok; ++half, ++it) {
-                    ok = acquire(it, half ? w_bytes : w_bytes + acts_bytes);
-                    if (!ok) break;
-                    uint8_t* st = smem + slot_of(it) * C_::STAGE_BYTES;
-                    load_stage_weights<C_>(st, &full[slot_of(it)], &p.tmGU, &p.tmGUE, (row0 + half * p.I) / 16, 2 * s,
-                                           pol_stream);
-                    if (!half) moe_load_acts<C_>(st, &full[slot_of(it)], &p.tmX, 0, p.strips, s, pol_keep);
-                }
-            }
-            // The down phase: the first stages' weights before the wait for h.
-            auto weights2 = [&](int u, int i) {
-                const int tile = u / S2, s = u % S2;
-                load_stage_weights<C_>(smem + slot_of(i) * C_::STAGE_BYTES, &full[slot_of(i)], &p.tmD, &p.tmDE,
-                                       (sh.list[s / Se] * p.H + tile * kTileM) / 16, 2 * (s % Se), pol_stream);
-            };
-            auto acts2 = [&](int u, int i) {
-                const int s = u % S2;
-                moe_load_acts<C_>(smem + slot_of(i) * C_::STAGE_BYTES, &full[slot_of(i)], &p.tmH, s / Se, p.strips,
-                                  s % Se, pol_keep);
-            };
-            int ahead = 0;
-            while (ok && ahead < STAGES && b2 + ahead < e2) {
-                ok = acquire(it + ahead, w_bytes + acts_bytes);
-                if (ok) {
-                    weights2(b2 + ahead, it + ahead);
-                    ++ahead;
-                }
-            }
-            if (ok && b2 < e2) {
-                ok = moe_wait(p.bar, base, bar_h, (uint32_t)grid);
-                SPMM24_STAMP(5);
-                ptx::fence_proxy_async_global();
-                if (ok) {
-                    for (int i = 0; i < ahead; ++i) acts2(b2 + i, it + i);
-                    for (int i = ahead; b2 + i < e2 && ok; ++i) {
-                        if (!(ok = acquire(it + i, w_bytes + acts_bytes))) break;
-                        weights2(b2 + i, it + i);
-                        acts2(b2 + i, it + i);
+            // The walks over units keep their place without divisions: one thread
+            // issues every load, and has 0.4 us a stage to keep up with HBM.
+#pragma unroll 1
+            for (int g = 0; g < n_groups && ok; ++g) {
+                const MoeRuns runs = runs1_of(g);
+                const int b = runs.begin(cta), e = runs.begin(cta + 1);
+                int s = b % S1, i_tile = b / S1 % i_tiles, slot = first_of(g) + b / S1 / i_tiles;
+                for (int u = b; u < e && ok; ++u) {
+                    const int row0 = sh.list[slot] * 2 * p.I + i_tile * kTileM;
+                    for (int half = 0; half < 2; ++half, ++it) {
+                        ok = acquire(it, half ? w_bytes : w_bytes + acts_bytes);
+                        if (!ok) break;
+                        uint8_t* st = smem + slot_of(it) * C_::STAGE_BYTES;
+                        load_stage_weights<C_>(st, &full[slot_of(it)], &p.tmGU, &p.tmGUE, (row0 + half * p.I) / 16, 2 * s,
+                                               pol_stream);
+                        if (!half) moe_load_acts<C_>(st, &full[slot_of(it)], &p.tmX, 0, p.strips, s, pol_keep);
+                    }
+                    if (++s == S1) {
+                        s = 0;
+                        if (++i_tile == i_tiles) {
+                            i_tile = 0;
+                            ++slot;
+                        }
                     }
                 }
+            }
+#pragma unroll 1
+            for (int g = 0; g < n_groups && ok; ++g) {
+                const MoeRuns runs = runs2_of(g);
+                const int b = runs.begin(cta), n = runs.begin(cta + 1) - b;
+                if (n <= 0) continue;
+                const int first = first_of(g), count = count_of(g);
+                struct Walk {
+                    int tile, slot, s;
+                };
+                auto step = [&](Walk& w) {
+                    if (++w.s < Se) return;
+                    w.s = 0;
+                    if (++w.slot < first + count) return;
+                    w.slot = first;
+                    ++w.tile;
+                };
+                const int in_tile = b % (count * Se);
+                Walk ww{b / (count * Se), first + in_tile / Se, in_tile % Se}, wa = ww;  // weights, activations
+                auto weights = [&](int i) {
+                    load_stage_weights<C_>(smem + slot_of(i) * C_::STAGE_BYTES, &full[slot_of(i)], &p.tmD, &p.tmDE,
+                                           (sh.list[ww.slot] * p.H + ww.tile * kTileM) / 16, 2 * ww.s, pol_stream);
+                    step(ww);
+                };
+                auto acts = [&](int i) {
+                    moe_load_acts<C_>(smem + slot_of(i) * C_::STAGE_BYTES, &full[slot_of(i)], &p.tmH, wa.slot, p.strips,
+                                      wa.s, pol_keep);
+                    step(wa);
+                };
+                // the first stages' weights before the wait for h
+                int ahead = 0;
+                while (ok && ahead < min(STAGES, n)) {
+                    ok = acquire(it + ahead, w_bytes + acts_bytes);
+                    if (ok) weights(it + ahead++);
+                }
+                if (ok) ok = moe_wait(p.bar, base, h_done(g), (uint32_t)grid);
+                if (g == 0) SPMM24_STAMP(5);
+                for (int i = 0; i < ahead && ok; ++i) acts(it + i);
+                for (int i = ahead; i < n && ok; ++i) {
+                    if (!(ok = acquire(it + i, w_bytes + acts_bytes))) break;
+                    weights(it + i);
+                    acts(it + i);
+                }
+                it += n;
             }
             if (!ok)  // gave up: let the copies in flight land before the block ends
                 for (int i = max(0, issued - STAGES); i < issued; ++i)
@@ -680,7 +739,7 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
         // -------------------------------------------------- MMA issuer
         const uint32_t smem_base = ptx::smem_u32(smem), fmt = p.bf16 ? kIdescBf16 : 0u;
         int it = 0, j = 0;
-        bool ok = true;
+        bool ok = n_active > 0;
         // waits until accumulator pair j & 1 has been read; false: give up
         auto begin_acc = [&]() {
             if (j >= 2) {
@@ -707,51 +766,62 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
                                           smem_base + acts % STAGES * C_::STAGE_BYTES,
                                           tmem_base + C_::META_COL + C_::META_STRIDE * (i % STAGES), d, accumulate, fmt);
         };
-        for (int u = b1; u < e1 && ok;) {
-            const int s0 = u % S1, s1 = min(S1, s0 + e1 - u);
-            if (!(ok = begin_acc())) break;
-            const uint32_t d = tmem_base + (uint32_t)((j & 1) * 2 * N_TILE);
-            for (int s = s0; s < s1 && ok; ++s, it += 2) {
-                for (int half = 0; half < 2; ++half) {
-                    if (!(ok = wait_full(it + half))) break;
-                    if (lane == 0 && it + half == 0) SPMM24_STAMP(1);
-                    if (2 * s + 1 >= gu_groups)
-                        patch_tail_metadata<C_>(smem + (it + half) % STAGES * C_::STAGE_BYTES, lane);
-                    if (lane == 0) {
-                        stage(it + half, it, d + (uint32_t)(half * N_TILE), s > s0);
-                        if (half) {  // the up product was the last to read the gate slot's activations
-                            ptx::tc_commit(&empty[it % STAGES]);
-                            ptx::tc_commit(&empty[(it + 1) % STAGES]);
+        auto end_acc = [&]() {
+            if (lane == 0) ptx::tc_commit(&acc_full[j & 1]);
+            __syncwarp();
+            ++j;
+        };
+#pragma unroll 1
+        for (int g = 0; g < n_groups && ok; ++g) {
+            const MoeRuns runs = runs1_of(g);
+            const int e = runs.begin(cta + 1);
+            for (int u = runs.begin(cta); u < e && ok;) {
+                const int s0 = u % S1, s1 = min(S1, s0 + e - u);
+                if (!(ok = begin_acc())) break;
+                const uint32_t d = tmem_base + (uint32_t)((j & 1) * 2 * N_TILE);
+                for (int s = s0; s < s1 && ok; ++s, it += 2) {
+                    for (int half = 0; half < 2; ++half) {
+                        if (!(ok = wait_full(it + half))) break;
+                        if (lane == 0 && it + half == 0) SPMM24_STAMP(1);
+                        if (2 * s + 1 >= gu_groups)
+                            patch_tail_metadata<C_>(smem + (it + half) % STAGES * C_::STAGE_BYTES, lane);
+                        if (lane == 0) {
+                            stage(it + half, it, d + (uint32_t)(half * N_TILE), s > s0);
+                            if (half) {  // the up product was the last to read the gate slot's activations
+                                ptx::tc_commit(&empty[it % STAGES]);
+                                ptx::tc_commit(&empty[(it + 1) % STAGES]);
+                            }
                         }
+                        __syncwarp();
+                    }
+                }
+                if (!ok) break;
+                end_acc();
+                u += s1 - s0;
+            }
+        }
+        if (lane == 0) SPMM24_STAMP(2);
+#pragma unroll 1
+        for (int g = 0; g < n_groups && ok; ++g) {
+            const MoeRuns runs = runs2_of(g);
+            const int e = runs.begin(cta + 1);
+            for (int u = runs.begin(cta); u < e && ok;) {  // a segment ends with its expert: the epilogue weighs each
+                const int s0 = u % Se, s1 = min(Se, s0 + e - u);
+                if (!(ok = begin_acc())) break;
+                const uint32_t d = tmem_base + (uint32_t)((j & 1) * 2 * N_TILE);
+                for (int s = s0; s < s1; ++s, ++it) {
+                    if (!(ok = wait_full(it))) break;
+                    if (2 * s + 1 >= d_groups) patch_tail_metadata<C_>(smem + it % STAGES * C_::STAGE_BYTES, lane);
+                    if (lane == 0) {
+                        stage(it, it, d, s > s0);
+                        ptx::tc_commit(&empty[it % STAGES]);
                     }
                     __syncwarp();
                 }
+                if (!ok) break;
+                end_acc();
+                u += s1 - s0;
             }
-            if (!ok) break;
-            if (lane == 0) ptx::tc_commit(&acc_full[j & 1]);
-            __syncwarp();
-            ++j;
-            u += s1 - s0;
-        }
-        if (lane == 0) SPMM24_STAMP(2);
-        for (int u = b2; u < e2 && ok;) {  // a segment ends with its expert: the epilogue weighs each on its own
-            const int s0 = u % Se, s1 = min(Se, s0 + e2 - u);
-            if (!(ok = begin_acc())) break;
-            const uint32_t d = tmem_base + (uint32_t)((j & 1) * 2 * N_TILE);
-            for (int s = s0; s < s1; ++s, ++it) {
-                if (!(ok = wait_full(it))) break;
-                if (2 * s + 1 >= d_groups) patch_tail_metadata<C_>(smem + it % STAGES * C_::STAGE_BYTES, lane);
-                if (lane == 0) {
-                    stage(it, it, d, s > s0);
-                    ptx::tc_commit(&empty[it % STAGES]);
-                }
-                __syncwarp();
-            }
-            if (!ok) break;
-            if (lane == 0) ptx::tc_commit(&acc_full[j & 1]);
-            __syncwarp();
-            ++j;
-            u += s1 - s0;
         }
         if (lane == 0) SPMM24_STAMP(7);
     } else {
@@ -776,84 +846,36 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
             if (lane == 0) ptx::mbar_arrive(&acc_empty[j & 1]);
             ++j;
         };
-        for (int u = b1; u < e1;) {
-            const int tile = u / S1, s0 = u % S1, s1 = min(S1, s0 + e1 - u);
-            u += s1 - s0;
-            uint32_t v[2 * N_TILE];  // gate, up
-            wait_acc();
-            moe_read_acc<2 * N_TILE>(tmem_row + (uint32_t)((j & 1) * 2 * N_TILE), v);
-            ptx::tmem_wait_ld();
-            release_acc();
-            if (s1 - s0 < S1) {
-                moe_put_partial<N_TILE>(p, v, row, (size_t)cta * 2 + (b1 < tile * S1 ? 1 : 0), tag);
-                continue;
-            }
-            const int slot = tile / i_tiles, e = sh.list[slot], r = tile % i_tiles * kTileM + row;
-            const bool live = r < p.I;
-            if constexpr (I8) {
-                const float gs = live ? p.gu_scale[(size_t)e * 2 * p.I + r] : 0.f;
-                const float us = live ? p.gu_scale[(size_t)e * 2 * p.I + p.I + r] : 0.f;
-                const uint32_t mask = sh.mask[e];
-#pragma unroll
-                for (int t = 0; t < N_TILE; ++t) {
-                    if (!(mask >> t & 1u)) continue;
-                    const float xs = sh.xscale[t];
-                    const float h = live ? moe_activate(int8_value((int)v[t], gs, xs), p.act) *
-                                               int8_value((int)v[N_TILE + t], us, xs)
-                                         : 0.f;
-                    if (live) __stcg(p.h32 + ((size_t)slot * p.T + t) * p.I + r, h);
-                    // bits order as magnitudes, NaN above all
-                    const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(h) & 0x7fffffffu);
-                    if (lane == 0) atomicMax(p.amax + slot * kMoeMaxTokens + t, m);
-                }
-            } else if (live) {
-#pragma unroll
-                for (int s = 0; s < N_TILE / 8; ++s) {
-                    if (s >= p.strips) break;
-                    uint32_t w[4];
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const int t = 8 * s + 2 * q;
-                        w[q] = pack2(moe_activate(__uint_as_float(v[t]), p.act) * __uint_as_float(v[N_TILE + t]),
-                                     moe_activate(__uint_as_float(v[t + 1]), p.act) * __uint_as_float(v[N_TILE + t + 1]),
-                                     p.bf16);
-                    }
-                    *reinterpret_cast<uint4*>(p.h16 + (((size_t)slot * p.strips + s) * p.I + r) * 8) =
-                        make_uint4(w[0], w[1], w[2], w[3]);
-                }
-            }
-        }
-        // The tiles that this CTA shares, first and last of its run.  A warp
-        // takes 32 rows and one or two pairs of tokens at a time.
-        constexpr int PAIRS = N_TILE / 16, BATCH = N_TILE == 16 ? 8 : 4;
-        auto shared_tiles = [&](int b, int e, int stages, const MoeRuns& runs, auto&& f) {
-            if (b >= e) return;
-            const int t0 = b / stages, t1 = (e - 1) / stages;
-            for (int t = t0; t <= t1; t += max(1, t1 - t0)) {
-                if (max(b, t * stages) == t * stages && min(e, (t + 1) * stages) == (t + 1) * stages) continue;
-                const MoeTile tile(runs, t, stages);
-                const int n = tile.c1 - tile.c0 + 1, i = cta - tile.c0;
-                f(t, tile, kTileM * i / n, kTileM * (i + 1) / n);
-            }
+        // all epilogue threads: wait for the launch's n-th grid barrier
+        auto wait_grid = [&](uint32_t n) {
+            if (threadIdx.x == 64) sh.last = ok && moe_wait(p.bar, base, n, (uint32_t)grid) ? 1u : 0u;
+            ptx::named_barrier(kBarEpi, kEpiThreads);
+            ok = ok && sh.last != 0u;
+            ptx::named_barrier(kBarEpi, kEpiThreads);
+            __threadfence();
         };
-        shared_tiles(b1, e1, S1, runs1, [&](int t, const MoeTile& tile, int r0, int r1) {
-            const int slot = t / i_tiles, e = sh.list[slot], blocks = (r1 - r0 + 31) / 32;
-            const int units = blocks * ((p.T + 2 * PAIRS - 1) / (2 * PAIRS));
-            const uint32_t mask = sh.mask[e];
-            for (int w = warp - 2; w < units; w += kEpiThreads / 32) {
-                const int rt = r0 + w % blocks * 32 + lane, t0 = w / blocks * 2 * PAIRS;  // row of the tile, first token
-                const int r = t % i_tiles * kTileM + rt;
-                const bool live = rt < r1 && r < p.I;
-                int col[2 * PAIRS];
-#pragma unroll
-                for (int n = 0; n < PAIRS; ++n) {
-                    // past the last token: its own columns again
-                    const int c = t0 + 2 * n < p.T ? t0 + 2 * n : t0;
-                    col[n] = c;
-                    col[PAIRS + n] = N_TILE + c;
+        // The tiles of a run: finished by the CTAs that share them, an equal
+        // part of the rows each.  A warp takes 32 rows and PAIRS pairs of tokens
+        // at a time, the loads of BATCH partials in flight: a gate / up tile of
+        // many tokens is shared by two or three CTAs, one of few tokens and a
+        // down tile by more.
+        constexpr int PAIRS = N_TILE == 16 ? 1 : 4, BATCH1 = N_TILE == 16 ? 8 : 2, BATCH2 = N_TILE == 16 ? 8 : 4;
+#pragma unroll 1
+        for (int g = 0; g < n_groups && n_active > 0; ++g) {
+            const MoeRuns runs = runs1_of(g);
+            const int b = runs.begin(cta), end = runs.begin(cta + 1), first = first_of(g);
+            if constexpr (I8) {  // the run's channel scales into L2, ahead of their use under a full stream
+                for (int t = b / S1; b < end && t * S1 < end; ++t) {
+                    const int r = t % i_tiles * kTileM + (int)(threadIdx.x & 3u) * 32;
+                    const float* at = p.gu_scale + (size_t)sh.list[first + t / i_tiles] * 2 * p.I + r;
+                    if (threadIdx.x < 64 + 8 && r < p.I) ptx::prefetch_l2(threadIdx.x & 4u ? at + p.I : at);
                 }
-                uint32_t v[4 * PAIRS];  // gate values, up values
-                moe_sum_partials<2 * PAIRS, BATCH, I8>(p, runs1, tile, col, min(rt, kTileM - 1), tag, v, ok);
+            }
+            for (int u = b; u < end;) {
+                const int tile = u / S1, s0 = u % S1, s1 = min(S1, s0 + end - u);
+                u += s1 - s0;
+                const int slot = first + tile / i_tiles, e = sh.list[slot], r = tile % i_tiles * kTileM + row;
+                const bool live = r < p.I;
                 float gs = 0.f, us = 0.f;
                 if constexpr (I8) {
                     if (live) {
@@ -861,76 +883,155 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
                         us = p.gu_scale[(size_t)e * 2 * p.I + p.I + r];
                     }
                 }
+                const uint32_t mask = sh.mask[e];
+                uint32_t v[2 * N_TILE];  // gate, up
+                wait_acc();
+                moe_read_acc<2 * N_TILE>(tmem_row + (uint32_t)((j & 1) * 2 * N_TILE), v);
+                ptx::tmem_wait_ld();
+                release_acc();
+                if (s1 - s0 < S1) {
+                    moe_put_partial<N_TILE>(p.part + (size_t)(2 * cta + (b < tile * S1 ? 1 : 0)) * kMoeSlotWords, v, row,
+                                            moe_pairs(mask), tag + (uint32_t)g);
+                    continue;
+                }
+                if constexpr (I8) {
 #pragma unroll
-                for (int n = 0; n < PAIRS; ++n) {
-                    if (t0 + 2 * n >= p.T) break;
-                    float h[2];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int tok = t0 + 2 * n + i;
-                        const uint32_t g = v[2 * n + i], u = v[2 * PAIRS + 2 * n + i];
-                        if constexpr (I8) {
-                            h[i] = 0.f;
-                            if (!(mask >> tok & 1u)) continue;
-                            const float xs = sh.xscale[tok];
-                            if (live) {
-                                h[i] = moe_activate(int8_value((int)g, gs, xs), p.act) * int8_value((int)u, us, xs);
-                                __stcg(p.h32 + ((size_t)slot * p.T + tok) * p.I + r, h[i]);
-                            }
-                            const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(h[i]) & 0x7fffffffu);
-                            if (lane == 0) atomicMax(p.amax + slot * kMoeMaxTokens + tok, m);
-                        } else {
-                            h[i] = moe_activate(__uint_as_float(g), p.act) * __uint_as_float(u);
-                        }
+                    for (int t = 0; t < N_TILE; ++t) {
+                        if (!(mask >> t & 1u)) continue;
+                        const float xs = sh.xscale[t];
+                        const float h = live ? moe_activate(int8_value((int)v[t], gs, xs), p.act) *
+                                                   int8_value((int)v[N_TILE + t], us, xs)
+                                             : 0.f;
+                        if (live) __stcg(p.h32 + ((size_t)slot * p.T + t) * p.I + r, h);
+                        // bits order as magnitudes, NaN above all
+                        const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(h) & 0x7fffffffu);
+                        if (lane == 0) atomicMax(p.amax + slot * kMoeMaxTokens + t, m);
                     }
-                    if constexpr (!I8) {
-                        const int tok = t0 + 2 * n;
-                        if (live)
-                            *reinterpret_cast<uint32_t*>(p.h16 + (((size_t)slot * p.strips + tok / 8) * p.I + r) * 8 +
-                                                         tok % 8) = pack2(h[0], h[1], p.bf16);
+                } else if (live) {
+#pragma unroll
+                    for (int s = 0; s < N_TILE / 8; ++s) {
+                        if (s >= p.strips) break;
+                        uint32_t w[4];
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const int t = 8 * s + 2 * q;
+                            w[q] = pack2(
+                                moe_activate(__uint_as_float(v[t]), p.act) * __uint_as_float(v[N_TILE + t]),
+                                moe_activate(__uint_as_float(v[t + 1]), p.act) * __uint_as_float(v[N_TILE + t + 1]),
+                                p.bf16);
+                        }
+                        *reinterpret_cast<uint4*>(p.h16 + (((size_t)slot * p.strips + s) * p.I + r) * 8) =
+                            make_uint4(w[0], w[1], w[2], w[3]);
                     }
                 }
             }
-        });
-        if (threadIdx.x == 64) SPMM24_STAMP(4);
-        // h is in place: this CTA's share
-        if (n_active > 0) {
+            // shared tiles: the first and the last of the run
+            for (int t = b / S1; b < end && t * S1 < end; t += max(1, (end - 1) / S1 - t)) {
+                if (b <= t * S1 && end >= (t + 1) * S1) continue;
+                const MoeTile tile(runs, t, S1);
+                const int shares = tile.c1 - tile.c0 + 1, mine = cta - tile.c0;
+                const int r0 = kTileM * mine / shares, r1 = kTileM * (mine + 1) / shares, blocks = (r1 - r0 + 31) / 32;
+                const int slot = first + t / i_tiles, e = sh.list[slot];
+                const uint32_t mask = sh.mask[e], pairs = moe_pairs(mask);
+                const int units = blocks * ((__popc(pairs) + PAIRS - 1) / PAIRS);
+                for (int w = warp - 2; w < units; w += kEpiThreads / 32) {
+                    const int rt = r0 + w % blocks * 32 + lane, r = t % i_tiles * kTileM + rt;  // row of the tile, of I
+                    const bool live = rt < r1 && r < p.I;
+                    float gs = 0.f, us = 0.f;
+                    if constexpr (I8) {
+                        if (live) {
+                            gs = p.gu_scale[(size_t)e * 2 * p.I + r];
+                            us = p.gu_scale[(size_t)e * 2 * p.I + p.I + r];
+                        }
+                    }
+                    uint32_t m = pairs;
+                    for (int n = w / blocks * PAIRS; n > 0; --n) m &= m - 1u;
+                    int col[2 * PAIRS], tok0[PAIRS];
+#pragma unroll
+                    for (int n = 0; n < PAIRS; ++n) {
+                        tok0[n] = m ? 2 * (__ffs((int)m) - 1) : -1;  // the pair's first token
+                        col[n] = m ? tok0[n] : col[0];               // none left: the first one's columns again
+                        col[PAIRS + n] = N_TILE + col[n];
+                        m &= m - 1u;
+                    }
+                    uint32_t v[4 * PAIRS];  // gate values, up values
+                    moe_sum_partials<2 * PAIRS, BATCH1, I8>(
+                        shares, [&](int i) { return p.part + (size_t)tile.slot(runs, tile.c0 + i) * kMoeSlotWords; }, col,
+                        min(rt, kTileM - 1), tag + (uint32_t)g, v, ok);
+#pragma unroll
+                    for (int n = 0; n < PAIRS; ++n) {
+                        if (tok0[n] < 0) break;
+                        float h[2];
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const int tok = tok0[n] + i;
+                            const uint32_t gv = v[2 * n + i], uv = v[2 * PAIRS + 2 * n + i];
+                            if constexpr (I8) {
+                                h[i] = 0.f;
+                                if (!(mask >> tok & 1u)) continue;
+                                const float xs = sh.xscale[tok];
+                                if (live) {
+                                    h[i] = moe_activate(int8_value((int)gv, gs, xs), p.act) * int8_value((int)uv, us, xs);
+                                    __stcg(p.h32 + ((size_t)slot * p.T + tok) * p.I + r, h[i]);
+                                }
+                                const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(h[i]) & 0x7fffffffu);
+                                if (lane == 0) atomicMax(p.amax + slot * kMoeMaxTokens + tok, top);
+                            } else {
+                                h[i] = moe_activate(__uint_as_float(gv), p.act) * __uint_as_float(uv);
+                            }
+                        }
+                        if constexpr (!I8) {
+                            if (live)
+                                *reinterpret_cast<uint32_t*>(
+                                    p.h16 + (((size_t)slot * p.strips + tok0[n] / 8) * p.I + r) * 8 + tok0[n] % 8) =
+                                    pack2(h[0], h[1], p.bf16);
+                        }
+                    }
+                }
+            }
+            if (threadIdx.x == 64) SPMM24_STAMP(4);
+            // the group's h is in place, this CTA's share of it
             if constexpr (!I8) ptx::fence_proxy_async_global();  // h is read by TMA
-            __threadfence();
             ptx::named_barrier(kBarEpi, kEpiThreads);
             if (threadIdx.x == 64 && ok) moe_arrive(p.bar, (uint32_t)grid);
-        }
-        if constexpr (I8) {
-            if (n_active > 0) {
-                // round h: (slot, token) rows in pieces of 512 values, a block each
-                if (threadIdx.x == 64) sh.last = ok && moe_wait(p.bar, base, barriers + 1u, (uint32_t)grid) ? 1u : 0u;
-                ptx::named_barrier(kBarEpi, kEpiThreads);
-                ok = ok && sh.last != 0u;
-                ptx::named_barrier(kBarEpi, kEpiThreads);
-                __threadfence();
-                {
-                    const int pieces = (p.I + 511) / 512, units = ok ? n_active * p.T * pieces : 0;
-                    for (int w = cta; w < units; w += grid) {
-                        const int piece = w % pieces, pair = w / pieces, slot = pair / p.T, t = pair % p.T;
-                        if (!(sh.mask[sh.list[slot]] >> t & 1u)) continue;
-                        const int c = piece * 512 + (threadIdx.x - 64) * 4;
-                        if (c >= p.I) continue;
-                        const float a = __uint_as_float(__ldcg(p.amax + slot * kMoeMaxTokens + t));
-                        const float inv = 127.f / a;
+            if constexpr (I8) {
+                // round h, once every row's largest value is known: (token,
+                // choice) rows in pieces of 512 values, four pieces in flight
+                wait_grid(barriers + 2u * (uint32_t)g + 1u);
+                constexpr int AHEAD = 4;
+                const int pieces = (p.I + 511) / 512, units = ok ? p.T * p.k * pieces : 0;
+                for (int w0 = cta; w0 < units; w0 += AHEAD * grid) {
+                    float4 h[AHEAD];
+                    float a[AHEAD];
+                    size_t at[AHEAD];
+#pragma unroll
+                    for (int n = 0; n < AHEAD; ++n) {
+                        const int w = w0 + n * grid, i = w / pieces, c = w % pieces * 512 + (threadIdx.x - 64) * 4;
+                        const int e = w < units ? sh.ids[i] : -1, slot = e < 0 ? 0 : sh.slot[e], t = i / p.k;
+                        a[n] = -1.f;
+                        if (e < 0 || (slot >= nA) != (g == 1) || c >= p.I) continue;
+                        at[n] = ((size_t)slot * p.T + t) * p.I + c;
+                        a[n] = __uint_as_float(__ldcg(p.amax + slot * kMoeMaxTokens + t));
+                        h[n] = __ldcg(reinterpret_cast<const float4*>(p.h32 + at[n]));
+                    }
+#pragma unroll
+                    for (int n = 0; n < AHEAD; ++n) {
+                        if (a[n] == -1.f) continue;
+                        const float inv = 127.f / a[n];
                         // else the row is zero (or below 1e-36), infinite or NaN: zeros, times its scale
                         const bool finite = inv > 0.f && inv <= 3.402823466e38f;
-                        const float4 h = __ldcg(reinterpret_cast<const float4*>(p.h32 + (size_t)pair * p.I + c));
-                        const float hv[4] = {h.x, h.y, h.z, h.w};
+                        const float hv[4] = {h[n].x, h[n].y, h[n].z, h[n].w};
                         uint32_t q[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) q[i] = finite ? (uint32_t)__float2int_rn(hv[i] * inv) : 0u;
-                        *reinterpret_cast<uint32_t*>(p.hq + (size_t)pair * p.I + c) = pack4(q[0], q[1], q[2], q[3]);
+                        *reinterpret_cast<uint32_t*>(p.hq + at[n]) = pack4(q[0], q[1], q[2], q[3]);
                     }
-                    ptx::fence_proxy_async_global();  // hq is read by TMA
-                    __threadfence();
-                    ptx::named_barrier(kBarEpi, kEpiThreads);
-                    if (threadIdx.x == 64 && ok) moe_arrive(p.bar, (uint32_t)grid);
                 }
+                ptx::fence_proxy_async_global();  // hq is read by TMA
+                ptx::named_barrier(kBarEpi, kEpiThreads);
+                if (threadIdx.x == 64 && ok) moe_arrive(p.bar, (uint32_t)grid);
+            } else if (g + 1 < n_groups) {
+                wait_grid(h_done(g));  // the next group's partials take the same slots
             }
         }
         const bool vec = (p.T % 8 == 0) && ((reinterpret_cast<uintptr_t>(p.y) & 15u) == 0) &&
@@ -948,75 +1049,107 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
                 epilogue_store8(p.y, f, p.epi, gm, c, p.H, p.T, vec, plain);
             }
         };
-        for (int u = b2; u < e2;) {
-            const int tile = u / S2, s0 = u % S2, s1 = min(S2, s0 + e2 - u);
-            uint32_t y[N_TILE];
+        uint64_t* const part2 = p.part + (size_t)kMoeMaxCtas * 2 * kMoeSlotWords;  // the first group's down partials
+#pragma unroll 1
+        for (int g = 0; g < n_groups && n_active > 0; ++g) {
+            const MoeRuns runs = runs2_of(g);
+            const int b = runs.begin(cta), end = runs.begin(cta + 1), first = first_of(g), S2 = count_of(g) * Se;
+            for (int u = b; u < end;) {
+                const int tile = u / S2, s0 = u % S2, s1 = min(S2, s0 + end - u);
+                uint32_t y[N_TILE];
 #pragma unroll
-            for (int t = 0; t < N_TILE; ++t) y[t] = 0u;
-            for (int s = s0; s < s1;) {
-                const int slot = s / Se, e = sh.list[slot];
-                // this expert's weight of token `lane` (the same expert twice: the sum)
-                float w = 0.f, scale = 1.f;
-                const uint32_t mask = sh.mask[e];
-                if (lane < p.T)
-                    for (int i = 0; i < p.k; ++i)
-                        if (sh.ids[lane * p.k + i] == e) w += sh.weights[lane * p.k + i];
-                if constexpr (I8) {
-                    if (mask >> lane & 1u) w *= __uint_as_float(__ldcg(p.amax + slot * kMoeMaxTokens + lane)) / 127.f;
-                    const int gm = tile * kTileM + row;
-                    scale = gm < p.H ? p.d_scale[(size_t)e * p.H + gm] : 0.f;
-                }
-                uint32_t v[N_TILE];
-                wait_acc();
-                moe_read_acc<N_TILE>(tmem_row + (uint32_t)((j & 1) * 2 * N_TILE), v);
-                ptx::tmem_wait_ld();
-                release_acc();
-#pragma unroll
-                for (int t = 0; t < N_TILE; ++t) {
-                    const float wt = __shfl_sync(0xffffffffu, w, t);
-                    const float d = I8 ? (float)(int)v[t] * scale : __uint_as_float(v[t]);
-                    if (mask >> t & 1u) y[t] = __float_as_uint(fmaf(wt, d, __uint_as_float(y[t])));
-                }
-                s = min(s1, (slot + 1) * Se);
-            }
-            u += s1 - s0;
-            if (s1 - s0 < S2)
-                moe_put_partial<N_TILE>(p, y, row, (size_t)cta * 2 + (b2 < tile * S2 ? 1 : 0), tag + 1u);
-            else
-                finish(y, tile);
-        }
-        shared_tiles(b2, e2, S2, runs2, [&](int t, const MoeTile& tile, int r0, int r1) {
-            const int cols = p.epi.packed ? 8 * p.strips : p.T, blocks = (r1 - r0 + 31) / 32;
-            const int units = blocks * ((cols + 2 * PAIRS - 1) / (2 * PAIRS));
-            for (int w = warp - 2; w < units; w += kEpiThreads / 32) {
-                const int rt = r0 + w % blocks * 32 + lane, t0 = w / blocks * 2 * PAIRS, gm = t * kTileM + rt;
-                int col[PAIRS];
-#pragma unroll
-                for (int n = 0; n < PAIRS; ++n) col[n] = t0 + 2 * n < p.T ? t0 + 2 * n : 0;
-                uint32_t v[2 * PAIRS];
-                moe_sum_partials<PAIRS, BATCH, false>(p, runs2, tile, col, min(rt, kTileM - 1), tag + 1u, v, ok);
-                if (rt >= r1 || gm >= p.H) continue;
-#pragma unroll
-                for (int i = 0; i < 2 * PAIRS; ++i) {
-                    const int tok = t0 + i;
-                    if (tok >= cols) break;
-                    const size_t at = c_offset(p.epi, gm, tok, p.H, p.T);
-                    float y[1] = {__uint_as_float(v[i])};
-                    if (!plain) {
-                        epilogue_pre<1>(y, p.epi, gm);
-                        if (p.epi.residual && tok < p.T) y[0] += elem_to_f32(p.epi.residual[at], p.epi.bf16);
+                for (int t = 0; t < N_TILE; ++t) y[t] = 0u;
+                for (int s = s0; s < s1;) {
+                    const int slot = first + s / Se, e = sh.list[slot];
+                    // this expert's weight of token `lane` (the same expert twice: the sum)
+                    float w = 0.f, scale = 1.f;
+                    const uint32_t mask = sh.mask[e];
+                    if (lane < p.T)
+                        for (int i = 0; i < p.k; ++i)
+                            if (sh.ids[lane * p.k + i] == e) w += sh.weights[lane * p.k + i];
+                    if constexpr (I8) {
+                        if (mask >> lane & 1u) w *= __uint_as_float(__ldcg(p.amax + slot * kMoeMaxTokens + lane)) / 127.f;
+                        const int gm = tile * kTileM + row;
+                        scale = gm < p.H ? p.d_scale[(size_t)e * p.H + gm] : 0.f;
                     }
-                    p.y[at] = tok < p.T ? f32_to_elem(y[0], p.epi.bf16) : (uint16_t)0;
+                    uint32_t v[N_TILE];
+                    wait_acc();
+                    moe_read_acc<N_TILE>(tmem_row + (uint32_t)((j & 1) * 2 * N_TILE), v);
+                    ptx::tmem_wait_ld();
+                    release_acc();
+#pragma unroll
+                    for (int t = 0; t < N_TILE; ++t) {
+                        const float wt = __shfl_sync(0xffffffffu, w, t);
+                        const float d = I8 ? (float)(int)v[t] * scale : __uint_as_float(v[t]);
+                        if (mask >> t & 1u) y[t] = __float_as_uint(fmaf(wt, d, __uint_as_float(y[t])));
+                    }
+                    s = min(s1, (s / Se + 1) * Se);
+                }
+                u += s1 - s0;
+                if (n_groups == 1 && s1 - s0 == S2) {
+                    finish(y, tile);
+                    continue;
+                }
+                // h_tiles <= grid where there are two groups: a run meets two tiles at most
+                const size_t slot = 2 * cta + (b < tile * S2 ? 1 : 0);
+                moe_put_partial<N_TILE>(g == 0 ? part2 + slot * (kMoeSlotWords / 2) : p.part + slot * kMoeSlotWords, y, row,
+                                        (1u << (p.T + 1) / 2) - 1u, tag + 2u);
+            }
+        }
+        if (n_active > 0) {
+            // the last group's run says whose tiles are whose; the first group's
+            // partials come first in the sum
+            const MoeRuns runs = runs2_of(n_groups - 1), runs_a = runs2_of(0);
+            const int b = runs.begin(cta), end = runs.begin(cta + 1), S2 = count_of(n_groups - 1) * Se;
+            for (int t = b / S2; b < end && t * S2 < end; ++t) {
+                if (n_groups == 1 && b <= t * S2 && end >= (t + 1) * S2) continue;
+                const MoeTile tile(runs, t, S2), tile_a(runs_a, t, nA * Se);
+                const int shares = tile.c1 - tile.c0 + 1, mine = cta - tile.c0;
+                const int before = n_groups == 2 ? tile_a.c1 - tile_a.c0 + 1 : 0;
+                const int r0 = kTileM * mine / shares, r1 = kTileM * (mine + 1) / shares, blocks = (r1 - r0 + 31) / 32;
+                const int cols = p.epi.packed ? 8 * p.strips : p.T;
+                const int units = blocks * ((cols + 2 * PAIRS - 1) / (2 * PAIRS));
+                auto slot = [&](int i) -> const uint64_t* {
+                    if (i < before) return part2 + (size_t)tile_a.slot(runs_a, tile_a.c0 + i) * (kMoeSlotWords / 2);
+                    const size_t at = tile.slot(runs, tile.c0 + i - before);
+                    return n_groups == 1 ? part2 + at * (kMoeSlotWords / 2) : p.part + at * kMoeSlotWords;
+                };
+                for (int w = warp - 2; w < units; w += kEpiThreads / 32) {
+                    const int rt = r0 + w % blocks * 32 + lane, t0 = w / blocks * 2 * PAIRS, gm = t * kTileM + rt;
+                    int col[PAIRS];
+#pragma unroll
+                    for (int n = 0; n < PAIRS; ++n) col[n] = t0 + 2 * n < p.T ? t0 + 2 * n : 0;
+                    uint32_t v[2 * PAIRS];
+                    moe_sum_partials<PAIRS, BATCH2, false>(before + shares, slot, col, min(rt, kTileM - 1), tag + 2u, v, ok);
+                    if (rt >= r1 || gm >= p.H) continue;
+                    if constexpr (PAIRS == 4) {
+                        float y[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) y[i] = __uint_as_float(v[i]);
+                        epilogue_store8(p.y, y, p.epi, gm, t0, p.H, p.T, vec, plain);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 2 * PAIRS; ++i) {
+                            const int tok = t0 + i;
+                            if (tok >= cols) break;
+                            const size_t at = c_offset(p.epi, gm, tok, p.H, p.T);
+                            float y[1] = {__uint_as_float(v[i])};
+                            if (!plain) {
+                                epilogue_pre<1>(y, p.epi, gm);
+                                if (p.epi.residual && tok < p.T) y[0] += elem_to_f32(p.epi.residual[at], p.epi.bf16);
+                            }
+                            p.y[at] = tok < p.T ? f32_to_elem(y[0], p.epi.bf16) : (uint16_t)0;
+                        }
+                    }
                 }
             }
-        });
-        if (threadIdx.x == 64) SPMM24_STAMP(6);
-        if (n_active == 0 && !sh.dead) {  // no token has an expert
+        } else if (!sh.dead) {  // no token has an expert
             uint32_t y[N_TILE];
 #pragma unroll
             for (int t = 0; t < N_TILE; ++t) y[t] = 0u;
             for (int tile = cta; tile < h_tiles; tile += grid) finish(y, tile);
         }
+        if (threadIdx.x == 64) SPMM24_STAMP(6);
     }
 
     ptx::tc_fence_before();
