@@ -85,7 +85,7 @@ struct MoeParams {
     SPMM24_TRACE_FIELD
 };
 
-constexpr int kMoeSharedBytes = 6400;
+constexpr int kMoeSharedBytes = 7168;
 constexpr int moe_stages(int n_tile, bool i8) { return n_tile == 16 ? 9 : i8 ? 7 : 8; }
 
 template <int N_TILE, bool I8>
@@ -109,6 +109,7 @@ struct MoeShared {
     uint16_t list[kMoeMaxExperts];               // experts in use, in increasing order
     uint8_t slot[kMoeMaxExperts];                // an expert's place there
     float xscale[kMoeMaxTokens];
+    uint32_t hmax[4][kMoeMaxTokens];             // int8: largest |h| (bits) in this CTA's rows, its run's first experts
     uint32_t red[kMoeWarps][8];
     uint32_t top[kMoeMaxTokens];
     uint32_t tmem, base, epoch, n_active, last, dead;
@@ -163,8 +164,8 @@ struct MoeRuns {
 // values of this layer are no load, and h is rounded after them.
 __device__ __forceinline__ float moe_activate(float y, int act) {
     if (act == kActRelu) return y > 0.f || y != y ? y : 0.f;
-    if (act == kActSilu) return y / (1.f + __expf(-y));
-    if (act == kActGelu) return y / (1.f + __expf(-1.5957691216057308f * (y + 0.044715f * y * y * y)));
+    if (act == kActSilu) return __fdividef(y, 1.f + __expf(-y));
+    if (act == kActGelu) return __fdividef(y, 1.f + __expf(-1.5957691216057308f * (y + 0.044715f * y * y * y)));
     return y;
 }
 
@@ -242,7 +243,8 @@ __device__ __forceinline__ uint32_t moe_key(float v) {
 // themselves down.  A thread per (token, expert), each against all: choosing
 // one after another is a chain of warp reductions (T = 8, E = 64, k = 8: 6.6 us
 // against 1 for this).  l, key: [T][pitch] logits and keys in shared memory,
-// padded with keys 0; l is left holding exp(l - largest).  All threads.
+// padded with keys 0 and -inf; l is left holding exp(l - largest).  All
+// threads.
 __device__ __forceinline__ void moe_top_k(const MoeParams& p, MoeShared& sh, float* l, const uint32_t* key, int pitch,
                                           bool publish) {
     const int n = p.T * p.E;
@@ -251,7 +253,7 @@ __device__ __forceinline__ void moe_top_k(const MoeParams& p, MoeShared& sh, flo
         const uint4* row = reinterpret_cast<const uint4*>(key + t * pitch);
         const uint32_t mine = key[t * pitch + e];
         int place = 0;
-#pragma unroll 2
+#pragma unroll 4
         for (int g = 0; g < pitch / 4; ++g) {
             const uint4 v = row[g];
             place += (v.x > mine || (v.x == mine && 4 * g < e)) + (v.y > mine || (v.y == mine && 4 * g + 1 < e)) +
@@ -264,10 +266,7 @@ __device__ __forceinline__ void moe_top_k(const MoeParams& p, MoeShared& sh, flo
         }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-        const int t = i / p.E, at = t * pitch + i - t * p.E;
-        l[at] = expf(l[at] - __uint_as_float(sh.top[t]));
-    }
+    for (int i = threadIdx.x; i < p.T * pitch; i += kThreads) l[i] = expf(l[i] - __uint_as_float(sh.top[i / pitch]));
     __syncthreads();
     for (int i = threadIdx.x; i < p.T * p.k; i += kThreads) {
         const int t = i / p.k;
@@ -275,8 +274,15 @@ __device__ __forceinline__ void moe_top_k(const MoeParams& p, MoeShared& sh, flo
         float sum = 0.f;
         if (p.norm)
             for (int j = 0; j < p.k; ++j) sum += lt[sh.ids[t * p.k + j]];
-        else
-            for (int e = 0; e < p.E; ++e) sum += lt[e];
+        else {
+            float4 s4 = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+            for (int e = 0; e < pitch; e += 4) {
+                const float4 x = *reinterpret_cast<const float4*>(lt + e);
+                s4 = make_float4(s4.x + x.x, s4.y + x.y, s4.z + x.z, s4.w + x.w);
+            }
+            sum = (s4.x + s4.y) + (s4.z + s4.w);
+        }
         const float w = lt[sh.ids[i]] / sum;
         sh.weights[i] = w;
         if (publish) {
@@ -398,6 +404,18 @@ __device__ __forceinline__ uint32_t moe_add(uint32_t a, uint32_t b) {
     return I8 ? a + b : __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
 }
 
+// int8: one warp's largest |h| of a token, to shared memory for the first four
+// experts of the CTA's run: global atomics stall behind a full weight stream
+// (0.5 us each), so there is one per token and expert, at the end of the run.
+__device__ __forceinline__ void moe_note_max(const MoeParams& p, MoeShared& sh, int slot, int nth, int t, float h) {
+    // bits order as magnitudes, NaN above all
+    const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(h) & 0x7fffffffu);
+    if ((threadIdx.x & 31u) == 0u) {
+        if (nth < 4) atomicMax(&sh.hmax[nth][t], m);
+        else atomicMax(p.amax + slot * kMoeMaxTokens + t, m);
+    }
+}
+
 // Two 64-bit words {value, tag, value, tag}: each word is read as it was
 // written, so a word with the right tag holds its value -- the partial needs no
 // fence, flag or counter (with those, a shared tile cost 5 us; so 2).
@@ -449,21 +467,26 @@ __device__ __forceinline__ uint32_t moe_pairs(uint32_t mask) {
 
 // Sums NP column pairs (the words of columns col[n], col[n] + 1) of one row
 // over `count` partials, BATCH of them in flight at once; slot(i): the i-th
-// partial's words.
+// partial's words.  fold: the warp's lanes are 8 rows by 4 parts of the
+// partials, whose sums lanes 0-7 then add in order -- for tiles of many
+// partials, which each hold few rows of.  The order of the sum depends on the
+// sizes and the routing alone.
 template <int NP, int BATCH, bool INT, class Slot>
 __device__ __forceinline__ void moe_sum_partials(int count, Slot&& slot, const int (&col)[NP], int row, uint32_t tag,
-                                                 uint32_t (&sum)[2 * NP], bool& ok) {
+                                                 bool fold, uint32_t (&sum)[2 * NP], bool& ok) {
+    const int part = fold ? (int)(threadIdx.x & 31u) >> 3 : 0;
+    const int first = fold ? count * part / 4 : 0, last = fold ? count * (part + 1) / 4 : count;
 #pragma unroll
     for (int n = 0; n < 2 * NP; ++n) sum[n] = 0u;
     uint64_t t0 = 0;
 #pragma unroll 1
-    for (int c = 0; c < count; c += BATCH) {
+    for (int c = first; c < last; c += BATCH) {
         uint64_t x[BATCH][2 * NP];
         for (uint32_t polls = 1;; ++polls) {
             bool there = true;
 #pragma unroll
             for (int i = 0; i < BATCH; ++i) {
-                if (c + i >= count) break;
+                if (c + i >= last) break;
                 const uint64_t* at = slot(c + i) + (size_t)row * 2;
 #pragma unroll
                 for (int n = 0; n < NP; ++n) moe_get2(at + (size_t)col[n] * kTileM, x[i][2 * n], x[i][2 * n + 1]);
@@ -472,7 +495,7 @@ __device__ __forceinline__ void moe_sum_partials(int count, Slot&& slot, const i
             for (int i = 0; i < BATCH; ++i)
 #pragma unroll
                 for (int n = 0; n < 2 * NP; ++n)
-                    there = there && (c + i >= count || (uint32_t)(x[i][n] >> 32) == tag);
+                    there = there && (c + i >= last || (uint32_t)(x[i][n] >> 32) == tag);
             if (there || !ok) break;
             ptx::nanosleep_ns(100);  // polls of every CTA at once would crowd out what they wait for
             if ((polls & 255u) == 0u) {
@@ -486,12 +509,20 @@ __device__ __forceinline__ void moe_sum_partials(int count, Slot&& slot, const i
         }
 #pragma unroll
         for (int i = 0; i < BATCH; ++i)
-            if (c + i < count) {
+            if (c + i < last) {
 #pragma unroll
                 for (int n = 0; n < 2 * NP; ++n) sum[n] = moe_add<INT>(sum[n], (uint32_t)x[i][n]);
             }
     }
     ok = __all_sync(0xffffffffu, ok);
+    if (fold) {
+#pragma unroll
+        for (int n = 0; n < 2 * NP; ++n) {
+            const uint32_t own = sum[n];
+#pragma unroll
+            for (int i = 1; i < 4; ++i) sum[n] = moe_add<INT>(sum[n], __shfl_down_sync(0xffffffffu, own, 8 * i));
+        }
+    }
 }
 
 template <int N_TILE, bool I8>
@@ -592,7 +623,7 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
             for (int s = 1; s < kMoeMaxShares; ++s)
                 if (s < p.logit_shares) sum += v[s];
             key[i] = e < p.E ? moe_key(sum) : 0u;
-            l[i] = sum;
+            l[i] = e < p.E ? sum : -INFINITY;
         }
         __syncthreads();
         moe_top_k(p, sh, l, key, pitch, cta == 0);
@@ -633,7 +664,9 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
     // little work: gate / up of A, of B, down of A, of B.
     const bool split = n_active > 1 && h_tiles <= grid &&
                        (long long)n_active * i_tiles * S1 >= (long long)kMoeSplitUnits * grid;
-    const int nA = split ? (n_active + 1) / 2 : n_active, n_groups = split ? 2 : 1;
+    // A is the larger: behind B's gate / up (two thirds of an expert's weights)
+    // A's barriers pass, behind A's down products B's
+    const int nA = split ? (2 * n_active + 1) / 3 : n_active, n_groups = split ? 2 : 1;
     // gate / up units (slot, 128 rows of I, stage), down units (128 rows of H, slot, stage) of one group
     auto first_of = [&](int g) { return g ? nA : 0; };
     auto count_of = [&](int g) { return g ? n_active - nA : nA; };
@@ -856,15 +889,18 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
         };
         // The tiles of a run: finished by the CTAs that share them, an equal
         // part of the rows each.  A warp takes 32 rows and PAIRS pairs of tokens
-        // at a time, the loads of BATCH partials in flight: a gate / up tile of
-        // many tokens is shared by two or three CTAs, one of few tokens and a
-        // down tile by more.
+        // at a time (of many partials 8 rows), the loads of BATCH partials in
+        // flight.
         constexpr int PAIRS = N_TILE == 16 ? 1 : 4, BATCH1 = N_TILE == 16 ? 8 : 2, BATCH2 = N_TILE == 16 ? 8 : 4;
 #pragma unroll 1
         for (int g = 0; g < n_groups && n_active > 0; ++g) {
             const MoeRuns runs = runs1_of(g);
             const int b = runs.begin(cta), end = runs.begin(cta + 1), first = first_of(g);
-            if constexpr (I8) {  // the run's channel scales into L2, ahead of their use under a full stream
+            const int slot0 = first + b / S1 / i_tiles;  // the run's first expert
+            if constexpr (I8) {
+                sh.hmax[warp - 2][lane] = 0u;
+                ptx::named_barrier(kBarEpi, kEpiThreads);
+                // the run's channel scales into L2, ahead of their use under a full stream
                 for (int t = b / S1; b < end && t * S1 < end; ++t) {
                     const int r = t % i_tiles * kTileM + (int)(threadIdx.x & 3u) * 32;
                     const float* at = p.gu_scale + (size_t)sh.list[first + t / i_tiles] * 2 * p.I + r;
@@ -903,9 +939,7 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
                                                    int8_value((int)v[N_TILE + t], us, xs)
                                              : 0.f;
                         if (live) __stcg(p.h32 + ((size_t)slot * p.T + t) * p.I + r, h);
-                        // bits order as magnitudes, NaN above all
-                        const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(h) & 0x7fffffffu);
-                        if (lane == 0) atomicMax(p.amax + slot * kMoeMaxTokens + t, m);
+                        moe_note_max(p, sh, slot, slot - slot0, t, h);
                     }
                 } else if (live) {
 #pragma unroll
@@ -930,13 +964,15 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
                 if (b <= t * S1 && end >= (t + 1) * S1) continue;
                 const MoeTile tile(runs, t, S1);
                 const int shares = tile.c1 - tile.c0 + 1, mine = cta - tile.c0;
-                const int r0 = kTileM * mine / shares, r1 = kTileM * (mine + 1) / shares, blocks = (r1 - r0 + 31) / 32;
+                const int r0 = kTileM * mine / shares, r1 = kTileM * (mine + 1) / shares;
+                const bool fold = shares > 4 && r1 - r0 <= 32 && __popc(moe_pairs(sh.mask[sh.list[first + t / i_tiles]])) < 4 * PAIRS;
+                const int rows = fold ? 8 : 32, blocks = (r1 - r0 + rows - 1) / rows;
                 const int slot = first + t / i_tiles, e = sh.list[slot];
                 const uint32_t mask = sh.mask[e], pairs = moe_pairs(mask);
                 const int units = blocks * ((__popc(pairs) + PAIRS - 1) / PAIRS);
                 for (int w = warp - 2; w < units; w += kEpiThreads / 32) {
-                    const int rt = r0 + w % blocks * 32 + lane, r = t % i_tiles * kTileM + rt;  // row of the tile, of I
-                    const bool live = rt < r1 && r < p.I;
+                    const int rt = r0 + w % blocks * rows + lane % rows, r = t % i_tiles * kTileM + rt;  // row of the tile, of I
+                    const bool live = lane < rows && rt < r1 && r < p.I;
                     float gs = 0.f, us = 0.f;
                     if constexpr (I8) {
                         if (live) {
@@ -957,7 +993,7 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
                     uint32_t v[4 * PAIRS];  // gate values, up values
                     moe_sum_partials<2 * PAIRS, BATCH1, I8>(
                         shares, [&](int i) { return p.part + (size_t)tile.slot(runs, tile.c0 + i) * kMoeSlotWords; }, col,
-                        min(rt, kTileM - 1), tag + (uint32_t)g, v, ok);
+                        min(rt, kTileM - 1), tag + (uint32_t)g, fold, v, ok);
 #pragma unroll
                     for (int n = 0; n < PAIRS; ++n) {
                         if (tok0[n] < 0) break;
@@ -974,8 +1010,7 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
                                     h[i] = moe_activate(int8_value((int)gv, gs, xs), p.act) * int8_value((int)uv, us, xs);
                                     __stcg(p.h32 + ((size_t)slot * p.T + tok) * p.I + r, h[i]);
                                 }
-                                const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(h[i]) & 0x7fffffffu);
-                                if (lane == 0) atomicMax(p.amax + slot * kMoeMaxTokens + tok, top);
+                                moe_note_max(p, sh, slot, slot - slot0, tok, h[i]);
                             } else {
                                 h[i] = moe_activate(__uint_as_float(gv), p.act) * __uint_as_float(uv);
                             }
@@ -991,7 +1026,14 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
             }
             if (threadIdx.x == 64) SPMM24_STAMP(4);
             // the group's h is in place, this CTA's share of it
-            if constexpr (!I8) ptx::fence_proxy_async_global();  // h is read by TMA
+            if constexpr (I8) {
+                ptx::named_barrier(kBarEpi, kEpiThreads);
+                const int slot = slot0 + warp - 2;
+                if (slot < first + count_of(g) && sh.hmax[warp - 2][lane])
+                    atomicMax(p.amax + slot * kMoeMaxTokens + lane, sh.hmax[warp - 2][lane]);
+            } else {
+                ptx::fence_proxy_async_global();  // h is read by TMA
+            }
             ptx::named_barrier(kBarEpi, kEpiThreads);
             if (threadIdx.x == 64 && ok) moe_arrive(p.bar, (uint32_t)grid);
             if constexpr (I8) {
@@ -1106,7 +1148,9 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
                 const MoeTile tile(runs, t, S2), tile_a(runs_a, t, nA * Se);
                 const int shares = tile.c1 - tile.c0 + 1, mine = cta - tile.c0;
                 const int before = n_groups == 2 ? tile_a.c1 - tile_a.c0 + 1 : 0;
-                const int r0 = kTileM * mine / shares, r1 = kTileM * (mine + 1) / shares, blocks = (r1 - r0 + 31) / 32;
+                const int r0 = kTileM * mine / shares, r1 = kTileM * (mine + 1) / shares;
+                const bool fold = before + shares > 4 && r1 - r0 <= 32 && p.T <= 6 * PAIRS;
+                const int rows = fold ? 8 : 32, blocks = (r1 - r0 + rows - 1) / rows;
                 const int cols = p.epi.packed ? 8 * p.strips : p.T;
                 const int units = blocks * ((cols + 2 * PAIRS - 1) / (2 * PAIRS));
                 auto slot = [&](int i) -> const uint64_t* {
@@ -1115,13 +1159,15 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
                     return n_groups == 1 ? part2 + at * (kMoeSlotWords / 2) : p.part + at * kMoeSlotWords;
                 };
                 for (int w = warp - 2; w < units; w += kEpiThreads / 32) {
-                    const int rt = r0 + w % blocks * 32 + lane, t0 = w / blocks * 2 * PAIRS, gm = t * kTileM + rt;
+                    const int rt = r0 + w % blocks * rows + lane % rows, t0 = w / blocks * 2 * PAIRS;
+                    const int gm = t * kTileM + rt;
                     int col[PAIRS];
 #pragma unroll
                     for (int n = 0; n < PAIRS; ++n) col[n] = t0 + 2 * n < p.T ? t0 + 2 * n : 0;
                     uint32_t v[2 * PAIRS];
-                    moe_sum_partials<PAIRS, BATCH2, false>(before + shares, slot, col, min(rt, kTileM - 1), tag + 2u, v, ok);
-                    if (rt >= r1 || gm >= p.H) continue;
+                    moe_sum_partials<PAIRS, BATCH2, false>(before + shares, slot, col, min(rt, kTileM - 1), tag + 2u, fold,
+                                                           v, ok);
+                    if (lane >= rows || rt >= r1 || gm >= p.H) continue;
                     if constexpr (PAIRS == 4) {
                         float y[8];
 #pragma unroll
