@@ -965,6 +965,10 @@ spmm24_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
                     chunk_out(r, c, gmr, gn, out);
                     *reinterpret_cast<uint4*>(p.C + (((size_t)(gn >> 3) * p.M + gmr) << 3)) = out;
                 }
+            } else if (I8 && !has_res && !vec_ok) {
+                const int ncols = min(C_::TILE_N, p.N - gn0);
+                for (int r = warp; r < kTileM && gm0 + r < p.M; r += kPairThreads / 32)
+                    copy_row_shifted(p.C + (size_t)(gm0 + r) * p.N + gn0, hst + (size_t)r * C_::C_PITCH, ncols, lane);
             } else {
                 // consecutive threads take consecutive chunks of a row
                 constexpr int RPP = kPairThreads / CH;  // rows per pass
@@ -1323,6 +1327,14 @@ spmm24_pair2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                     v = make_uint4(x[0], x[1], x[2], x[3]);
                 }
                 *reinterpret_cast<uint4*>(reinterpret_cast<__half*>(p.C) + (((size_t)(gn >> 3) * p.M + gm) << 3)) = v;
+            }
+        } else if (I8 && !((p.N % 8 == 0) && ((reinterpret_cast<uintptr_t>(p.C) & 15u) == 0))) {
+            const int gn0 = n_tile * C_::TILE_N, ncols = min(C_::TILE_N, p.N - gn0);
+            for (int r = warp; r < 2 * kTileM; r += kPairThreads / 32) {
+                const int gm = m_tile * C_::TILE_M + (r / kTileM) * 2 * kTileM + (int)rank * kTileM + r % kTileM;
+                if (gm < p.M)
+                    copy_row_shifted(p.C + (size_t)gm * p.N + gn0,
+                                     reinterpret_cast<const uint16_t*>(cst) + (size_t)r * C_::C_PITCH, ncols, lane);
             }
         } else if (etid < LPR * RPP) {
             const int chunk = etid % LPR;

@@ -191,6 +191,14 @@ def _stream_handle(stream) -> int | None:
     return int(stream.cuda_stream)
 
 
+def _current_stream(tensor) -> int:
+    """The handle of torch's current stream on the tensor's device (as an
+    integer: the Stream object costs 2 us)."""
+    import torch
+
+    return torch._C._cuda_getCurrentRawStream(tensor.device.index)
+
+
 # -------------------------------------------------------------- launch
 def launch(stream, compressed_a, b_packed, metadata, c, M: int, N: int, K: int, split_reduction=None,
            split_k: int = 0) -> int:
@@ -244,14 +252,14 @@ def quantize_int8(x, rows: int, cols: int, q=None, scale=None, bf16: bool = Fals
                   stream=None):
     """spmm24_quantize_int8: rows of 16-bit x (row-major with row stride ld, or
     packed strips) -> (q: rows x cols int8, scale: rows floats)."""
-    import torch
-
+    if q is None or scale is None:
+        import torch
     if q is None:
         q = torch.empty((rows, cols), dtype=torch.int8, device=x.device)
     if scale is None:
         scale = torch.empty(rows, dtype=torch.float32, device=x.device)
     if stream is None:
-        stream = torch.cuda.current_stream(x.device)
+        stream = _current_stream(x)
     rc = _lib.spmm24_quantize_int8(_stream_handle(stream), _ptr(x), rows, cols, ld,
                                    OUT_PACKED_B if packed else OUT_ROW_MAJOR, BF16 if bf16 else 0, _ptr(q), _ptr(scale))
     if rc != CUDA_SUCCESS:
