@@ -55,12 +55,12 @@ __device__ __forceinline__ void store8(int8_t* row, int k, int cols, uint2 q) {
     }
 }
 
-constexpr int kHeld = 4;  // groups of eight elements that a thread holds in registers
-
-// One row per block.  A thread's groups lie blockDim apart; what does not fit
-// in registers (rows of more than 32 blockDim elements) is read again, out of
-// L2.
-template <bool BF16, bool VEC>
+// One row per block.  A thread holds HELD groups of eight elements in
+// registers, blockDim apart; what does not fit (rows of more than 65536 elements)
+// is read again, out of L2.  HELD 4 up to 8192 columns, 8 above: 4096 x 4096 9.9
+// and 9.7 us, 148 x 4096 1.5 and 1.9; 4096 x 11008 28.6 and 25.4, 2048 x 28672
+// 46.1 and 36.4 (more bytes in flight for a row; fewer warps for a short one).
+template <bool BF16, bool VEC, int HELD>
 __global__ void __launch_bounds__(1024) quantize_rows_kernel(const uint16_t* __restrict__ x, long long ld, int cols,
                                                              int8_t* __restrict__ q, float* __restrict__ scale) {
     __shared__ uint32_t warp_max[32];
@@ -69,45 +69,53 @@ __global__ void __launch_bounds__(1024) quantize_rows_kernel(const uint16_t* __r
     const uint16_t* row = x + (long long)blockIdx.x * ld;
     int8_t* out = q + (long long)blockIdx.x * cols;
     const int groups = (cols + 7) / 8, step = blockDim.x;
-    uint4 v[kHeld];
+    uint4 v[HELD];
     uint32_t m = 0u;
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
+    for (int i = 0; i < HELD; ++i) {
         const int g = (int)threadIdx.x + i * step;
         v[i] = g < groups ? load8<VEC>(row, 8 * g, cols) : make_uint4(0u, 0u, 0u, 0u);
     }
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) m = vmaxu2(m, abs_max8(v[i]));
-    for (int g = (int)threadIdx.x + kHeld * step; g < groups; g += step) m = vmaxu2(m, abs_max8(load8<VEC>(row, 8 * g, cols)));
+    for (int i = 0; i < HELD; ++i) m = vmaxu2(m, abs_max8(v[i]));
+    for (int g = (int)threadIdx.x + HELD * step; g < groups; g += step) m = vmaxu2(m, abs_max8(load8<VEC>(row, 8 * g, cols)));
     const RowScale r = row_scale<BF16>(block_max(m, warp_max), threadIdx.x == 0 ? scale + blockIdx.x : nullptr);
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
+    for (int i = 0; i < HELD; ++i) {
         const int g = (int)threadIdx.x + i * step;
         if (g < groups) store8<VEC>(out, 8 * g, cols, quantize8<BF16>(v[i], r));
     }
-    for (int g = (int)threadIdx.x + kHeld * step; g < groups; g += step)
+    for (int g = (int)threadIdx.x + HELD * step; g < groups; g += step)
         store8<VEC>(out, 8 * g, cols, quantize8<BF16>(load8<VEC>(row, 8 * g, cols), r));
 }
 
-// One strip of eight rows (packed B: cols x 8 elements) per block.  A thread
-// takes eight consecutive columns of all eight rows: 128 bytes in, eight bytes
-// of each row out.  The first such group waits in registers, the others are
-// read again, out of L2.
+// One strip of eight rows (packed B: cols x 8 elements) per cluster, an equal
+// part of its columns per CTA; the CTAs exchange their eight maxima through
+// distributed shared memory.  A thread takes eight consecutive columns of all
+// eight rows: 128 bytes in, eight bytes of each row out.  The first such group
+// waits in registers, the others (more than 4096 columns a CTA) are read again,
+// out of L2.  (A column per lane, and a byte transpose across eight lanes for the
+// stores, measured the same.)
+constexpr int kMaxStripCtas = 8;
+
 template <bool BF16>
-__global__ void __launch_bounds__(1024) quantize_strips_kernel(const uint16_t* __restrict__ x, int rows, int cols,
-                                                               int8_t* __restrict__ q, float* __restrict__ scale) {
-    __shared__ uint32_t part[32][8];
-    __shared__ uint32_t top[8];
+__global__ void __launch_bounds__(512, 2) quantize_strips_kernel(const uint16_t* __restrict__ x, int rows, int cols,
+                                                              int8_t* __restrict__ q, float* __restrict__ scale) {
+    __shared__ uint32_t part[16][8];
+    __shared__ uint32_t tops[kMaxStripCtas][8];
+    __shared__ RowScale rs[8];
+    const int ctas = (int)ptx::cluster_nctarank(), rank = (int)ptx::cluster_ctarank();
     ptx::grid_dep_wait();
     if (threadIdx.x == 0) ptx::grid_dep_launch();
-    const uint4* strip = reinterpret_cast<const uint4*>(x) + (size_t)blockIdx.x * cols;  // one uint4 per column
-    const int groups = cols / 8, row0 = (int)blockIdx.x * 8;
+    const int strip_id = (int)blockIdx.x / ctas, row0 = strip_id * 8;
+    const uint4* strip = reinterpret_cast<const uint4*>(x) + (size_t)strip_id * cols;  // one uint4 per column
+    const int g0 = (int)((long long)(cols / 8) * rank / ctas), g1 = (int)((long long)(cols / 8) * (rank + 1) / ctas);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint4 v[8];
-    const bool first = (int)threadIdx.x < groups;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = first ? strip[8 * threadIdx.x + i] : make_uint4(0u, 0u, 0u, 0u);
     uint32_t m[4] = {0u, 0u, 0u, 0u};  // rows 2i (low) and 2i + 1 (high)
+    const int mine = g0 + (int)threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = mine < g1 ? strip[8 * mine + i] : make_uint4(0u, 0u, 0u, 0u);
     auto fold = [&](uint4 w) {
         m[0] = vmaxu2(m[0], w.x & 0x7fff7fffu);
         m[1] = vmaxu2(m[1], w.y & 0x7fff7fffu);
@@ -116,7 +124,7 @@ __global__ void __launch_bounds__(1024) quantize_strips_kernel(const uint16_t* _
     };
 #pragma unroll
     for (int i = 0; i < 8; ++i) fold(v[i]);
-    for (int c = 8 * (int)blockDim.x + (int)threadIdx.x; c < cols; c += (int)blockDim.x) fold(strip[c]);
+    for (int c = 8 * (g0 + (int)blockDim.x) + (int)threadIdx.x; c < 8 * g1; c += (int)blockDim.x) fold(strip[c]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const uint32_t lo = __reduce_max_sync(0xffffffffu, m[i] & 0xffffu);
@@ -127,22 +135,29 @@ __global__ void __launch_bounds__(1024) quantize_strips_kernel(const uint16_t* _
         }
     }
     __syncthreads();
+    if ((int)threadIdx.x < 8 * ctas) {  // this CTA's maxima into every CTA's slot of it
+        const int j = threadIdx.x & 7, to = threadIdx.x >> 3;
+        uint32_t t = 0u;
+        for (int w = 0; w < (int)blockDim.x / 32; ++w) t = max(t, part[w][j]);
+        ptx::st_cluster_u32(ptx::mapa_shared(ptx::smem_u32(&tops[rank][j]), (uint32_t)to), t);
+    }
+    ptx::cluster_sync();
     if (threadIdx.x < 8) {
         uint32_t t = 0u;
-        for (int w = 0; w < (int)(blockDim.x + 31) / 32; ++w) t = max(t, part[w][threadIdx.x]);
-        top[threadIdx.x] = t;
-        if (row0 + (int)threadIdx.x < rows) row_scale<BF16>(t, scale + row0 + threadIdx.x);
+        for (int c = 0; c < ctas; ++c) t = max(t, tops[c][threadIdx.x]);
+        const int row = row0 + (int)threadIdx.x;
+        rs[threadIdx.x] = row_scale<BF16>(t, rank == 0 && row < rows ? scale + row : nullptr);
     }
     __syncthreads();
-    for (int g = threadIdx.x; g < groups; g += blockDim.x) {
-        if (g != (int)threadIdx.x) {
+    for (int g = mine; g < g1; g += blockDim.x) {
+        if (g != mine) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = strip[8 * g + i];
         }
 #pragma unroll
         for (int pair = 0; pair < 4; ++pair) {
             uint32_t lo[8], hi[8];
-            const RowScale r0 = row_scale<BF16>(top[2 * pair], nullptr), r1 = row_scale<BF16>(top[2 * pair + 1], nullptr);
+            const RowScale r0 = rs[2 * pair], r1 = rs[2 * pair + 1];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const uint32_t w = pair == 0 ? v[i].x : pair == 1 ? v[i].y : pair == 2 ? v[i].z : v[i].w;
@@ -165,16 +180,21 @@ __global__ void __launch_bounds__(1024) quantize_strips_kernel(const uint16_t* _
 }
 
 template <class... KArgs, class... Args>
-cudaError_t launch(void (*kern)(KArgs...), unsigned blocks, unsigned threads, cudaStream_t stream, bool pdl, Args... args) {
+cudaError_t launch(void (*kern)(KArgs...), unsigned blocks, unsigned threads, unsigned cluster, cudaStream_t stream, bool pdl,
+                   Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(blocks, 1, 1);
     cfg.blockDim = dim3(threads, 1, 1);
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = pdl ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
 }
 
@@ -200,19 +220,31 @@ extern "C" cudaError_t spmm24_quantize_int8(cudaStream_t stream, const void* x, 
         if (cols % 8) return record_invalid("packed rows: cols must be a multiple of 8");
         if (((uintptr_t)x & 15u) || ((uintptr_t)q & 7u))
             return record_invalid("packed rows: x must be 16-byte and q 8-byte aligned");
-        const unsigned threads = (unsigned)(groups < 512 ? (groups + 31) / 32 * 32 : 512);
-        const unsigned blocks = (unsigned)(((long long)rows + 7) / 8);
-        return bf16 ? launch(quantize_strips_kernel<true>, blocks, threads, stream, pdl, xp, rows, cols, qp, scale)
-                    : launch(quantize_strips_kernel<false>, blocks, threads, stream, pdl, xp, rows, cols, qp, scale);
+        // CTAs per strip: eight where strips are few (64 elements a thread are 1.2
+        // us of arithmetic when one CTA has 4096 columns) or long (registers hold
+        // 4096 columns a CTA): 16 x 4096 5.4 us with one, 3.4 with eight; 509 x 4096
+        // 5.4 and 4.5; 4096 x 4096 15.1 and 20; 4096 x 11008 48 and 41.
+        const long long strips = ((long long)rows + 7) / 8;
+        unsigned ctas = kMaxStripCtas;
+        while (ctas > 1 && cols <= 4096 && (strips * ctas > 8 * 148 || groups < 64 * (int)ctas)) ctas /= 2;
+        const int each = (groups + (int)ctas - 1) / (int)ctas;
+        const unsigned threads = (unsigned)(each < 512 ? (each + 31) / 32 * 32 : 512);
+        if (strips * ctas > 0x7fffffffLL) return record_invalid("packed rows: too many rows");
+        const unsigned blocks = (unsigned)(strips * ctas);
+        return bf16 ? launch(quantize_strips_kernel<true>, blocks, threads, ctas, stream, pdl, xp, rows, cols, qp, scale)
+                    : launch(quantize_strips_kernel<false>, blocks, threads, ctas, stream, pdl, xp, rows, cols, qp, scale);
     }
     if (ld == 0) ld = cols;
     if (ld < cols) return record_invalid("ld must be 0 or at least cols");
     const bool vec = cols % 8 == 0 && ld % 8 == 0 && ((uintptr_t)x & 15u) == 0 && ((uintptr_t)q & 7u) == 0;
-    unsigned threads = (unsigned)((groups + 32 * kHeld - 1) / (32 * kHeld) * 32);
+    const int held = cols > 8192 ? 8 : 4;
+    unsigned threads = (unsigned)((groups + 32 * held - 1) / (32 * held) * 32);
     if (threads > 1024) threads = 1024;
-    if (bf16)
-        return vec ? launch(quantize_rows_kernel<true, true>, (unsigned)rows, threads, stream, pdl, xp, ld, cols, qp, scale)
-                   : launch(quantize_rows_kernel<true, false>, (unsigned)rows, threads, stream, pdl, xp, ld, cols, qp, scale);
-    return vec ? launch(quantize_rows_kernel<false, true>, (unsigned)rows, threads, stream, pdl, xp, ld, cols, qp, scale)
-               : launch(quantize_rows_kernel<false, false>, (unsigned)rows, threads, stream, pdl, xp, ld, cols, qp, scale);
+    auto go = [&](auto kern) { return launch(kern, (unsigned)rows, threads, 0u, stream, pdl, xp, ld, cols, qp, scale); };
+    if (held == 8) {
+        if (bf16) return vec ? go(quantize_rows_kernel<true, true, 8>) : go(quantize_rows_kernel<true, false, 8>);
+        return vec ? go(quantize_rows_kernel<false, true, 8>) : go(quantize_rows_kernel<false, false, 8>);
+    }
+    if (bf16) return vec ? go(quantize_rows_kernel<true, true, 4>) : go(quantize_rows_kernel<true, false, 4>);
+    return vec ? go(quantize_rows_kernel<false, true, 4>) : go(quantize_rows_kernel<false, false, 4>);
 }

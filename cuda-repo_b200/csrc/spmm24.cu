@@ -27,6 +27,7 @@
 #include "spmm24_kernel.cuh"
 #include "spmm24_grouped.cuh"
 #include "spmm24_moe.cuh"
+#include "spmm24_prefill.cuh"
 
 namespace spmm24 {
 
@@ -174,6 +175,7 @@ using Pair2C8 = Pair2Cfg<kPair2Stages, true>;
 using PairC8 = PairCfg<kPairStages, true>;
 using PairCI8 = PairCfg<kPairStages, true, 128, true>;
 using Pair2CI8 = Pair2Cfg<kPair2Stages, true, true>;
+using PrefillC = PrefillCfg<kPair2Stages>;
 // Stream-K variants: the scratch-array kernel of spmm24_launch_noalloc.
 using SV16 = StreamKVariant<16, 8>;
 using SV32 = StreamKVariant<32, 8>;
@@ -186,6 +188,7 @@ struct Plan {
     Path path;
     bool pair2;        // pair path with two M halves per pair (512 x 240 tiles)
     bool narrow;       // pair path with 256 x 128 tiles
+    bool persist;      // int8: the two-M-half pair's tiles on persistent pairs
     bool shallow;      // 4-stage ring, two CTAs per SM (narrow N only)
     int tile_n;
     int stages;
@@ -458,6 +461,28 @@ cudaError_t launch_cluster_int8(const Plan& pl, cudaStream_t stream, int dev, bo
                          stream, (unsigned)pl.split, pdl, ta, tb, te, kp);
 }
 
+cudaError_t launch_prefill_int8(const Plan& pl, cudaStream_t stream, int dev, bool pdl, const CUtensorMap& ta,
+                                const CUtensorMap& tb, const CUtensorMap& te, const PairParams& kp) {
+    auto kern = spmm24_prefill_int8_kernel<kPair2Stages>;
+    cudaError_t e = prepare(kern, PrefillC::SMEM_ALLOC, dev, kInt8Slot + 14);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)pl.grid, 1, 1);
+    cfg.blockDim = dim3((unsigned)kPrefillThreads, 1, 1);
+    cfg.dynamicSmemBytes = PrefillC::SMEM_ALLOC;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = pdl ? 1 : 0;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kern, ta, tb, te, kp, pl.m_tiles, pl.n_tiles);
+}
+
 template <class V>
 cudaError_t launch_streamk(const Plan& pl, cudaStream_t stream, int dev, bool pdl, const CUtensorMap& ta,
                            const CUtensorMap& tb, const CUtensorMap& te, const StreamKParams& kp, int idx) {
@@ -685,12 +710,44 @@ cudaError_t launch_impl(cudaStream_t stream, const void* A, const void* B, const
 // two-M-half pair (512 x 240) when its waves cost less and the epilogue has
 // no residual (pair2_ok).  The int8 SpMM (i8) has the same formats, stages and
 // plans, but for the two-M-half pair's tile of 512 x 224.
+
+// Persistent pairs (int8): the plan's waves of tiles against rounds of 512 x 224
+// tiles, by the times that the three kernels' tiles take (measured, K = 4096
+// and 11008, st stages of 256 K; one clock, so the ratios count): 8.1 + 0.38 st us
+// for a 256 x 256 tile, 8.8 + 0.69 st for a 512 x 224 one, and persistent 5.2 +
+// 0.665 st and 3 us at the start.  11008 x 4096 x 4096: 140 (256 x 256), 119.5
+// (512 x 224), 99 us; 4096^3: 57, 58, 50; 8192^3: 330, 271, 230; 4096 x 4096 x
+// 11008: 98, 107, 102 (the rule keeps 256 x 256).
+void maybe_persist(Plan& p, int M, int N, int sms) {
+    if (g_tune.pair2.load(std::memory_order_relaxed) == 0) return;  // override: no two-M-half tiles
+    const long long slots = std::max(1, sms / 2);
+    const long long m2 = (M + 4 * kTileM - 1) / (4 * kTileM), n2 = (N + Pair2CI8::TILE_N - 1) / Pair2CI8::TILE_N;
+    const long long rounds = (m2 * n2 + slots - 1) / slots;
+    if (rounds < 2) return;  // one tile per pair: nothing to overlap
+    const long long waves = ((long long)p.m_tiles * p.n_tiles * p.split + slots - 1) / slots;
+    // in units of 0.01 us; stages_total counts 256-K stages
+    const long long st = p.stages_total;
+    const long long cost = 300 + rounds * (520 + 67 * st);
+    const long long base = p.pair2 ? waves * (880 + 69 * st) : waves * (810 + 38 * st);
+    if (cost >= base && g_tune.pair2.load(std::memory_order_relaxed) != 1) return;
+    p.pair2 = p.persist = true;
+    p.split = 1;
+    p.tile_n = Pair2CI8::TILE_N;
+    p.stages = kPair2Stages;
+    p.smem = PrefillC::SMEM_ALLOC;
+    p.m_tiles = (int)m2;
+    p.n_tiles = (int)n2;
+    p.grid = 2 * (int)std::min(slots, m2 * n2);
+}
+
 template <class V>
 int fp8_smem(bool i8) {
     return i8 ? ClusterCfg<V::kTileN, V::kStages, true, true>::SMEM_ALLOC : ClusterCfg<V::kTileN, V::kStages, true>::SMEM_ALLOC;
 }
 
-Plan plan_fp8(int M, int N, int K, int split_k, int sms, bool pair2_ok, bool i8 = false) {
+// persist_ok: the persistent int8 kernel may be chosen (no residual; row-major C
+// with N % 8 == 0 and aligned, or packed).
+Plan plan_fp8(int M, int N, int K, int split_k, int sms, bool pair2_ok, bool i8 = false, bool persist_ok = false) {
     const int Kh = K / 2;
     Plan pl = make_plan(M, N, Kh, split_k, sms, Kh % 128 == 0, 5, false, false);
     if (pl.path == Path::kPair) {
@@ -698,6 +755,7 @@ Plan plan_fp8(int M, int N, int K, int split_k, int sms, bool pair2_ok, bool i8 
         if (pl.split == 1 && split_k <= 1 && pair2_ok)
             maybe_pair2(pl, M, N, sms, i8 ? Pair2CI8::TILE_N : Pair2C8::TILE_N, kPair2Stages,
                         i8 ? Pair2CI8::SMEM_ALLOC : Pair2C8::SMEM_ALLOC);
+        if (i8 && persist_ok && split_k <= 1) maybe_persist(pl, M, N, sms);
     } else if (pl.shallow) {
         pl.smem = pl.tile_n == 16 ? fp8_smem<CV16s>(i8) : fp8_smem<CV32s>(i8);
     } else {
@@ -741,7 +799,8 @@ cudaError_t launch_fp8_impl(cudaStream_t stream, const void* A, const void* B, c
     e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     const int Kh = K / 2;  // the 16-bit-equivalent K of the A bytes
-    Plan pl = plan_fp8(M, N, K, split_k, sm_count(dev), !epi.residual, i8);
+    const bool c_ok = epi.packed || (N % 8 == 0 && ((uintptr_t)C & 15u) == 0);
+    Plan pl = plan_fp8(M, N, K, split_k, sm_count(dev), !epi.residual, i8, !epi.residual && c_ok);
     const bool pair = pl.path == Path::kPair;
 
     CUtensorMap ta, tb, te;
@@ -789,6 +848,7 @@ cudaError_t launch_fp8_impl(cudaStream_t stream, const void* A, const void* B, c
         kp.mma_fmt = mma_fmt;
         kp.w_scale = w_scale;
         kp.x_scale = x_scale;
+        if (pl.persist) return launch_prefill_int8(pl, stream, dev, pdl, ta, tb, te, kp);
         if (pl.pair2)
             return i8 ? launch_pair2_fp8<true>(pl, stream, dev, pdl, ta, tb, te, kp)
                       : launch_pair2_fp8<false>(pl, stream, dev, pdl, ta, tb, te, kp);
@@ -1780,7 +1840,7 @@ extern "C" int spmm24_select_config_fp8(int M, int N, int K, int split_k, spmm24
 
 extern "C" int spmm24_select_config_int8(int M, int N, int K, int split_k, spmm24_config* out) {
     if (!out || M <= 0 || N <= 0 || K <= 0 || M % 16 || K % 128 || K > spmm24::kInt8MaxK || split_k < 0) return -1;
-    spmm24::fill_config(spmm24::plan_fp8(M, N, K, split_k, spmm24::current_sms(), true, true), 256, out);
+    spmm24::fill_config(spmm24::plan_fp8(M, N, K, split_k, spmm24::current_sms(), true, true, N % 8 == 0), 256, out);
     return 0;
 }
 

@@ -566,7 +566,7 @@ int spmm24_group_schedule(const int* M, const int* K, int count, int fp8, int sm
  * K of fp8 operands; K % 128 == 0), for an epilogue without a residual or a
  * packed output. */
 int spmm24_select_config_fp8(int M, int N, int K, int split_k, spmm24_config* out);
-/* The same for spmm24_launch_int8. */
+/* The same for spmm24_launch_int8 (row-major C, 16-byte aligned). */
 int spmm24_select_config_int8(int M, int N, int K, int split_k, spmm24_config* out);
 
 /* Row range of shard `index` of `parts` when an M x K layer is split along

@@ -229,6 +229,42 @@ def test_every_kernel_gives_the_same_bits(cuda_device, tuning, kw):
     assert np.array_equal(_run(cuda_device, M, N, K, bias=True, act=2, seed=3), want)
 
 
+# more 512 x 224 tiles than pairs of SMs: the persistent kernel, two and three
+# tiles a pair, one to five stages of K, ragged M and N
+@pytest.mark.parametrize("M,N,K,kw", [
+    (5120, 2048, 256, dict()), (5136, 2040, 512, dict(bf16=True, bias=True, act=2)),
+    (5008, 2008, 768, dict(packed=True, act=1, bias=True)), (5120, 2041, 1024, dict(packed=True, bf16=True)),
+    (11008, 2048, 1280, dict(alpha=0.5, act=3)), (5120, 2048, 512, dict(w=False, xs=False)),
+    (4624, 2240, 512, dict(flags=spmm24.STATIC_WEIGHTS)),
+], ids=lambda v: str(v) if isinstance(v, int) else "-".join(v))
+def test_persistent_tiles(cuda_device, tuning, M, N, K, kw):
+    tuning(pair2=1)
+    got = _run(cuda_device, M, N, K, seed=K, **kw)
+    tuning(pair2=0)  # the sums are exact: another kernel, the same bits
+    assert np.array_equal(_run(cuda_device, M, N, K, seed=K, **kw), got)
+
+
+def test_persistent_tiles_back_to_back(cuda_device):
+    """Launches that overlap (each reads what the one before wrote), many tiles each."""
+    import torch
+
+    M, N, K = 5120, 2048, 512
+    a, b = problem(M, N, K, 5)
+    vals, meta = spmm24.compress_a_int8(a, M, K)
+    dv, dm, db = _dev(vals, cuda_device), _dev(meta, cuda_device), _dev(b, cuda_device)
+    st = torch.cuda.current_stream(cuda_device)
+    scale = torch.ones(N, device=cuda_device)
+    outs = [torch.zeros(M, N, dtype=torch.float16, device=cuda_device) for _ in range(6)]
+    for i, c in enumerate(outs):
+        scale.fill_(2.0 ** -(8 + i))
+        assert spmm24.launch_int8(st, dv, db, dm, c, M, N, K, x_scale=scale, flags=spmm24.STATIC_WEIGHTS) == 0
+    torch.cuda.synchronize()
+    acc = torch.from_numpy(product(a, b)).to(cuda_device)
+    for i, c in enumerate(outs):
+        assert torch.equal(c, (acc * 2.0 ** -(8 + i)).to(torch.float32).to(torch.float16))
+    assert spmm24.device_status(0) == 0
+
+
 @pytest.mark.parametrize("split", range(1, 9))
 def test_splits_give_the_same_bits(cuda_device, split):
     want = _run(cuda_device, 272, 21, 2176, split=1, seed=4)
