@@ -959,7 +959,8 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
                     }
                 }
             }
-            // shared tiles: the first and the last of the run
+            // shared tiles: the first and the last of the run, their units dealt to the warps in turn
+            int dealt = 0;
             for (int t = b / S1; b < end && t * S1 < end; t += max(1, (end - 1) / S1 - t)) {
                 if (b <= t * S1 && end >= (t + 1) * S1) continue;
                 const MoeTile tile(runs, t, S1);
@@ -969,8 +970,9 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
                 const int rows = fold ? 8 : 32, blocks = (r1 - r0 + rows - 1) / rows;
                 const int slot = first + t / i_tiles, e = sh.list[slot];
                 const uint32_t mask = sh.mask[e], pairs = moe_pairs(mask);
-                const int units = blocks * ((__popc(pairs) + PAIRS - 1) / PAIRS);
-                for (int w = warp - 2; w < units; w += kEpiThreads / 32) {
+                const int units = blocks * ((__popc(pairs) + PAIRS - 1) / PAIRS), mine0 = (warp - 2 - dealt) & 3;
+                dealt += units;
+                for (int w = mine0; w < units; w += kEpiThreads / 32) {
                     const int rt = r0 + w % blocks * rows + lane % rows, r = t % i_tiles * kTileM + rt;  // row of the tile, of I
                     const bool live = lane < rows && rt < r1 && r < p.I;
                     float gs = 0.f, us = 0.f;
@@ -1143,6 +1145,7 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
             // partials come first in the sum
             const MoeRuns runs = runs2_of(n_groups - 1), runs_a = runs2_of(0);
             const int b = runs.begin(cta), end = runs.begin(cta + 1), S2 = count_of(n_groups - 1) * Se;
+            int dealt = 0;
             for (int t = b / S2; b < end && t * S2 < end; ++t) {
                 if (n_groups == 1 && b <= t * S2 && end >= (t + 1) * S2) continue;
                 const MoeTile tile(runs, t, S2), tile_a(runs_a, t, nA * Se);
@@ -1152,13 +1155,14 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
                 const bool fold = before + shares > 4 && r1 - r0 <= 32 && p.T <= 6 * PAIRS;
                 const int rows = fold ? 8 : 32, blocks = (r1 - r0 + rows - 1) / rows;
                 const int cols = p.epi.packed ? 8 * p.strips : p.T;
-                const int units = blocks * ((cols + 2 * PAIRS - 1) / (2 * PAIRS));
+                const int units = blocks * ((cols + 2 * PAIRS - 1) / (2 * PAIRS)), mine0 = (warp - 2 - dealt) & 3;
+                dealt += units;
                 auto slot = [&](int i) -> const uint64_t* {
                     if (i < before) return part2 + (size_t)tile_a.slot(runs_a, tile_a.c0 + i) * (kMoeSlotWords / 2);
                     const size_t at = tile.slot(runs, tile.c0 + i - before);
                     return n_groups == 1 ? part2 + at * (kMoeSlotWords / 2) : p.part + at * kMoeSlotWords;
                 };
-                for (int w = warp - 2; w < units; w += kEpiThreads / 32) {
+                for (int w = mine0; w < units; w += kEpiThreads / 32) {
                     const int rt = r0 + w % blocks * rows + lane % rows, t0 = w / blocks * 2 * PAIRS;
                     const int gm = t * kTileM + rt;
                     int col[PAIRS];

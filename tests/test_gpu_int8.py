@@ -64,13 +64,14 @@ def _random_bits(rows, cols, bf16, seed):
 
 @pytest.mark.parametrize("bf16", [False, True], ids=["fp16", "bf16"])
 @pytest.mark.parametrize("rows,cols", [(1, 1), (3, 7), (2, 8), (9, 31), (5, 256), (1, 1000), (130, 4096), (7, 11008),
-                                       (2, 40000), (3, 40001)])
+                                       (2, 40000), (3, 40001), (2, 70008), (1, 70001)])
 def test_quantize_rows(cuda_device, rows, cols, bf16):
     _check_quantize(cuda_device, _random_bits(rows, cols, bf16, rows + cols), bf16)
 
 
 @pytest.mark.parametrize("bf16", [False, True], ids=["fp16", "bf16"])
-@pytest.mark.parametrize("rows,cols", [(1, 8), (8, 64), (9, 256), (3, 4096), (17, 4104), (33, 11008)])
+@pytest.mark.parametrize("rows,cols", [(1, 8), (8, 64), (9, 256), (3, 4096), (17, 4104), (33, 11008), (9, 40008),
+                                       (1300, 264)])
 def test_quantize_strips(cuda_device, rows, cols, bf16):
     _check_quantize(cuda_device, _random_bits(rows, cols, bf16, rows + cols), bf16, packed=True)
 

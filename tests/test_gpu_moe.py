@@ -190,7 +190,7 @@ class Layer:
 
 SHAPES = [(1, 128, 128, 1, 1), (3, 1024, 640, 5, 2), (8, 256, 384, 64, 8), (9, 128, 256, 7, 3), (16, 384, 896, 4, 4),
           (17, 384, 640, 6, 2), (32, 512, 1408, 16, 4), (32, 256, 256, 256, 16), (2, 4096, 2048, 8, 2),
-          (24, 2176, 128, 33, 5)]
+          (24, 2176, 128, 33, 5), (2, 24576, 128, 3, 2), (1, 128, 8192, 5, 3), (11, 4096, 1408, 12, 3)]
 
 
 @pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "T%d-%dx%d-E%dk%d" % s)
