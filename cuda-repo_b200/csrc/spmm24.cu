@@ -98,9 +98,12 @@ bool encode(CUtensorMap* m, int rank, const void* base, const cuuint64_t* dims, 
     k.rank = rank;
     k.type = (int)type;
     k.swizzle = (int)swizzle;
-    uint64_t h = 1469598103934665603ull;  // FNV-1a over the key bytes
-    const unsigned char* kb = reinterpret_cast<const unsigned char*>(&k);
-    for (size_t i = 0; i < sizeof(k); ++i) h = (h ^ kb[i]) * 1099511628211ull;
+    // FNV-1a over the key's 8-byte words (byte by byte the three keys of a
+    // launch took 0.4 us of its 4.4 on the host)
+    static_assert(sizeof(k) % 8 == 0, "whole words");
+    uint64_t words[sizeof(k) / 8], h = 1469598103934665603ull;
+    std::memcpy(words, &k, sizeof(k));
+    for (uint64_t w : words) h = (h ^ w ^ (w >> 32)) * 1099511628211ull;
     MapEntry& slot = t_map_cache[(h ^ (h >> 29)) % kMapCacheSlots];
     if (slot.valid && std::memcmp(&slot.key, &k, sizeof(k)) == 0) {
         *m = slot.map;

@@ -967,6 +967,7 @@ spmm24_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
                 }
             } else if (I8 && !has_res && !vec_ok) {
                 const int ncols = min(C_::TILE_N, p.N - gn0);
+#pragma unroll 4
                 for (int r = warp; r < kTileM && gm0 + r < p.M; r += kPairThreads / 32)
                     copy_row_shifted(p.C + (size_t)(gm0 + r) * p.N + gn0, hst + (size_t)r * C_::C_PITCH, ncols, lane);
             } else {
@@ -1330,6 +1331,7 @@ spmm24_pair2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             }
         } else if (I8 && !((p.N % 8 == 0) && ((reinterpret_cast<uintptr_t>(p.C) & 15u) == 0))) {
             const int gn0 = n_tile * C_::TILE_N, ncols = min(C_::TILE_N, p.N - gn0);
+#pragma unroll 4
             for (int r = warp; r < 2 * kTileM; r += kPairThreads / 32) {
                 const int gm = m_tile * C_::TILE_M + (r / kTileM) * 2 * kTileM + (int)rank * kTileM + r % kTileM;
                 if (gm < p.M)

@@ -232,10 +232,10 @@ __device__ __forceinline__ void moe_router(const MoeParams& p, MoeShared& sh, in
 }
 
 // A logit's key: keys order as the logits do, NaN above all (it then makes
-// every weight of its token NaN); -0 and +0 are a tie.
+// every weight of its token NaN) and below 2^32 - 1; -0 and +0 are a tie.
 __device__ __forceinline__ uint32_t moe_key(float v) {
     const uint32_t b = __float_as_uint(v + 0.f);
-    return v != v ? 0xffffffffu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
+    return v != v ? 0xfffffffeu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 
 // Top k of every token, by rank: an expert's place is the number of its
@@ -256,8 +256,9 @@ __device__ __forceinline__ void moe_top_k(const MoeParams& p, MoeShared& sh, flo
 #pragma unroll 4
         for (int g = 0; g < pitch / 4; ++g) {
             const uint4 v = row[g];
-            place += (v.x > mine || (v.x == mine && 4 * g < e)) + (v.y > mine || (v.y == mine && 4 * g + 1 < e)) +
-                     (v.z > mine || (v.z == mine && 4 * g + 2 < e)) + (v.w > mine || (v.w == mine && 4 * g + 3 < e));
+            // before this one: the larger, and of the equal those to its left
+            place += (v.x >= mine + (4 * g >= e)) + (v.y >= mine + (4 * g + 1 >= e)) + (v.z >= mine + (4 * g + 2 >= e)) +
+                     (v.w >= mine + (4 * g + 3 >= e));
         }
         if (place < p.k) {
             sh.ids[t * p.k + place] = e;
