@@ -49,6 +49,8 @@
 // too short to hide them (a message through L2 takes 1-2 us while it is full),
 // and the last partials (3-4 us).
 #pragma once
+#include <cstddef>
+
 #include "int8_rows.cuh"
 #include "spmm24_common.cuh"
 
@@ -94,7 +96,8 @@ struct MoeParams {
     SPMM24_TRACE_FIELD
 };
 
-constexpr int kMoeSharedBytes = 7168;
+constexpr int kMoeSharedBytes = 6880 + 4 * 768;
+constexpr int kMoeKeptLogits = 768;
 constexpr int moe_stages(int n_tile, bool i8) { return n_tile == 16 ? 9 : i8 ? 7 : 8; }
 
 template <int N_TILE, bool I8>
@@ -122,8 +125,10 @@ struct MoeShared {
     uint32_t red[kMoeWarps][8];
     uint32_t top[kMoeMaxTokens];
     uint32_t tmem, base, epoch, n_active, last, dead;
+    alignas(16) float logits[kMoeKeptLogits];    // the logits, where they fit; read four at a time
 };
 static_assert(sizeof(MoeShared) <= kMoeSharedBytes, "MoeCfg reserves its bytes");
+static_assert(offsetof(MoeShared, logits) % 16 == 0, "read as float4");
 
 // ------------------------------------------------------------ grid barrier
 // One word that counts arrivals, `ctas` per barrier, and wraps at a multiple
@@ -252,10 +257,9 @@ __device__ __forceinline__ uint32_t moe_key(float v) {
 // themselves down.  A thread per (token, expert), each against all: choosing
 // one after another is a chain of warp reductions (T = 8, E = 64, k = 8: 6.6 us
 // against 1 for this).  l, key: [T][pitch] logits and keys in shared memory,
-// padded with keys 0 and -inf; l is left holding exp(l - largest).  All
-// threads.
-__device__ __forceinline__ void moe_top_k(const MoeParams& p, MoeShared& sh, float* l, const uint32_t* key, int pitch,
-                                          bool publish) {
+// padded with -inf and keys 0.  All threads.
+__device__ __forceinline__ void moe_top_k(const MoeParams& p, MoeShared& sh, const float* l, const uint32_t* key,
+                                          int pitch) {
     const int n = p.T * p.E;
     for (int i = threadIdx.x; i < n; i += kThreads) {
         const int t = i / p.E, e = i - t * p.E;
@@ -275,25 +279,32 @@ __device__ __forceinline__ void moe_top_k(const MoeParams& p, MoeShared& sh, flo
             atomicOr(&sh.mask[e], 1u << t);
         }
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < p.T * pitch; i += kThreads) l[i] = expf(l[i] - __uint_as_float(sh.top[i / pitch]));
-    __syncthreads();
-    for (int i = threadIdx.x; i < p.T * p.k; i += kThreads) {
+}
+
+// The chosen experts' weights, a thread for each, out of the logits l (EXP: out
+// of exp(l - largest)).  thread, threads: the caller's place among those that
+// take part.
+template <bool EXP>
+__device__ __forceinline__ void moe_weights(const MoeParams& p, MoeShared& sh, const float* l, int pitch, int thread,
+                                            int threads, bool publish) {
+    for (int i = thread; i < p.T * p.k; i += threads) {
         const int t = i / p.k;
         const float* lt = l + t * pitch;
+        const float top = __uint_as_float(sh.top[t]);
+        auto e_of = [&](float x) { return EXP ? x : expf(x - top); };
         float sum = 0.f;
-        if (p.norm)
-            for (int j = 0; j < p.k; ++j) sum += lt[sh.ids[t * p.k + j]];
-        else {
+        if (p.norm) {
+            for (int j = 0; j < p.k; ++j) sum += e_of(lt[sh.ids[t * p.k + j]]);
+        } else {
             float4 s4 = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+#pragma unroll 2
             for (int e = 0; e < pitch; e += 4) {
                 const float4 x = *reinterpret_cast<const float4*>(lt + e);
-                s4 = make_float4(s4.x + x.x, s4.y + x.y, s4.z + x.z, s4.w + x.w);
+                s4 = make_float4(s4.x + e_of(x.x), s4.y + e_of(x.y), s4.z + e_of(x.z), s4.w + e_of(x.w));
             }
             sum = (s4.x + s4.y) + (s4.z + s4.w);
         }
-        const float w = lt[sh.ids[i]] / sum;
+        const float w = e_of(lt[sh.ids[i]]) / sum;
         sh.weights[i] = w;
         if (publish) {
             if (p.ids) p.ids[i] = sh.ids[i];
@@ -550,7 +561,12 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int cta = (int)blockIdx.x, grid = (int)gridDim.x;
 
+    // The barrier's count before this CTA's first arrival, and the epoch: under
+    // way while the router runs.
+    uint32_t count0 = 0u, epoch0 = 0u;
     if (threadIdx.x == 0) {
+        count0 = ptx::ld_relaxed_gpu(p.bar);
+        epoch0 = ptx::ld_relaxed_gpu(p.epoch);
         SPMM24_STAMP(0);
         for (int s = 0; s < STAGES; ++s) {
             ptx::mbar_init(&full[s], 1);
@@ -561,9 +577,6 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
             ptx::mbar_init(&acc_empty[b], kEpiThreads / 32);
         }
         ptx::fence_mbarrier_init();
-        const uint32_t c = ptx::ld_acquire_gpu(p.bar);  // before this CTA's first arrival
-        sh.base = c - c % (uint32_t)grid;
-        sh.epoch = ptx::ld_acquire_gpu(p.epoch);
         sh.dead = 0u;
         ptx::prefetch_tmap(&p.tmGU);
         ptx::prefetch_tmap(&p.tmGUE);
@@ -597,6 +610,10 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
         if (p.bf16) moe_router<true>(p, sh, unit0, grid);
         else moe_router<false>(p, sh, unit0, grid);
     }
+    if (threadIdx.x == 0) {
+        sh.base = count0 - count0 % (uint32_t)grid;
+        sh.epoch = epoch0;
+    }
     if constexpr (I8) ptx::fence_proxy_async_global();  // xq is read by TMA
     __syncthreads();
     ptx::tc_fence_after();
@@ -614,12 +631,15 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
     }
 
     // --------------------------------------------------------- routing
-    if (I8 && threadIdx.x < p.T) sh.xscale[threadIdx.x] = __ldcg(p.xscale + threadIdx.x);
+    // The weights are not needed before the down products: where the logits are
+    // kept, the epilogue warps compute them behind the first weight stages.
+    const int pitch = (p.E + 3) / 4 * 4;
+    const bool kept = p.router && p.T * pitch <= kMoeKeptLogits;
     if (p.router) {
         // T x E logits and keys in the ring, which is still idle
-        const int pitch = (p.E + 3) / 4 * 4, n = p.T * pitch, logits = p.T * p.E;
+        const int n = p.T * pitch, logits = p.T * p.E;
         uint32_t* key = reinterpret_cast<uint32_t*>(smem);
-        float* l = reinterpret_cast<float*>(key + n);
+        float* l = kept ? sh.logits : reinterpret_cast<float*>(key + n);
 #pragma unroll 2
         for (int i = threadIdx.x; i < n; i += kThreads) {
             const int t = i / pitch, e = i - t * pitch;
@@ -636,7 +656,13 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
             l[i] = e < p.E ? sum : -INFINITY;
         }
         __syncthreads();
-        moe_top_k(p, sh, l, key, pitch, cta == 0);
+        moe_top_k(p, sh, l, key, pitch);
+        if (!kept) {
+            __syncthreads();
+            for (int i = threadIdx.x; i < n; i += kThreads) l[i] = expf(l[i] - __uint_as_float(sh.top[i / pitch]));
+            __syncthreads();
+            moe_weights<true>(p, sh, l, pitch, threadIdx.x, kThreads, cta == 0);
+        }
         ptx::fence_proxy_async_smem();  // before TMA writes the ring
     } else {
         for (int i = threadIdx.x; i < p.T * p.k; i += kThreads) {
@@ -901,6 +927,9 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
         // part of the rows each.  A warp takes 32 rows and PAIRS pairs of tokens
         // at a time (of many partials 8 rows), the loads of BATCH partials in
         // flight.
+        if (I8 && threadIdx.x - 64 < p.T) sh.xscale[threadIdx.x - 64] = __ldcg(p.xscale + threadIdx.x - 64);
+        if (kept) moe_weights<false>(p, sh, sh.logits, pitch, threadIdx.x - 64, kEpiThreads, cta == 0);
+        ptx::named_barrier(kBarEpi, kEpiThreads);
         constexpr int PAIRS = N_TILE == 16 ? 1 : 4, BATCH1 = N_TILE == 16 ? 8 : 2, BATCH2 = N_TILE == 16 ? 8 : 4;
 #pragma unroll 1
         for (int g = 0; g < n_groups && n_active > 0; ++g) {
