@@ -207,6 +207,7 @@ extern "C" cudaError_t spmm24_quantize_int8(cudaStream_t stream, const void* x, 
     clear_last_error();
     if (!x || !q || !scale) return record_invalid("null pointer");
     if (rows <= 0 || cols <= 0) return record_invalid("rows and cols must be positive");
+    if (cols > 1 << 30) return record_invalid("cols must be at most 2^30");  // the kernels' column indices run past it
     if (flags & ~(unsigned)(SPMM24_BF16 | SPMM24_NO_PDL)) return record_invalid("unknown flag");
     if (layout != SPMM24_OUT_ROW_MAJOR && layout != SPMM24_OUT_PACKED_B) return record_invalid("unknown input layout");
     if ((uintptr_t)x & 1u) return record_invalid("x must be 2-byte aligned");

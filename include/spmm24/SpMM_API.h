@@ -396,7 +396,8 @@ cudaError_t spmm24_launch_fp8(cudaStream_t stream, const void* values, const voi
  *           cols = its M), x 16-byte and q 8-byte aligned, cols % 8 == 0, ld 0
  *   flags   SPMM24_BF16 (x holds bf16), SPMM24_NO_PDL
  * q: rows x cols int8, row-major (the b_nk of spmm24_launch_int8); scale:
- * rows floats.  Asynchronous on `stream`. */
+ * rows floats; neither may overlap x.  cols is at most 2^30.  Asynchronous on
+ * `stream`. */
 cudaError_t spmm24_quantize_int8(cudaStream_t stream, const void* x, int rows, int cols, long long ld, int layout,
                                  unsigned flags, void* q, float* scale);
 /* Magnitude 2:4 prune of a row-major M x K int8 matrix in place (ties prefer
@@ -460,7 +461,8 @@ cudaError_t spmm24_launch_int8(cudaStream_t stream, const void* values, const vo
  *               (spmm24_device_status), zero it again.
  * flags: SPMM24_BF16, SPMM24_MOE_INT8; SPMM24_STATIC_WEIGHTS and SPMM24_NO_PDL
  * are accepted and change nothing (the kernel is launched cooperatively, in
- * stream order).  Allocates nothing.  Asynchronous on `stream`. */
+ * stream order).  y and the workspace overlap no other operand.  Allocates
+ * nothing.  Asynchronous on `stream`. */
 enum { SPMM24_MOE_INT8 = 32u };
 typedef struct spmm24_moe_layer {
     int tokens, hidden, inter, experts, top_k;

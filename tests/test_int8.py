@@ -100,7 +100,8 @@ def test_launch_refusals(kw, why):
     (dict(cols=-1), "positive"), (dict(flags=1), "flag"), (dict(layout=2), "layout"), (dict(x=0x1001), "aligned"),
     (dict(scale=0x3002), "aligned"), (dict(ld=99), "ld"), (dict(ld=-1), "ld"),
     (dict(layout=1, ld=100), "ld"), (dict(layout=1, cols=100), "multiple of 8"), (dict(layout=1, x=0x1008), "16-byte"),
-    (dict(layout=1, q=0x2004), "8-byte"),
+    (dict(layout=1, q=0x2004), "8-byte"), (dict(cols=(1 << 30) + 8), "2^30"), (dict(cols=2**31 - 1), "2^30"),
+    (dict(layout=1, cols=2**31 - 8), "2^30"),
 ])
 def test_quantize_refusals(kw, why):
     a = dict(x=0x1000, rows=4, cols=104, ld=0, layout=0, flags=0, q=0x2000, scale=0x3000) | kw
