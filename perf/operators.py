@@ -12,7 +12,6 @@ Three operators that a decode or prefill step of a 2:4-sparse model calls:
 library's entry points.  Weights are made once per layer, in dense form and
 in the library's packed form (SpMM_API.h documents both packed formats).
 """
-import functools
 import math
 import os
 import sys
@@ -24,7 +23,6 @@ own = False
 _TYPES = {"fp16": torch.float16, "bf16": torch.bfloat16}
 
 
-@functools.cache
 def _library():
     path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "cuda-repo_b200")
     if path not in sys.path:
