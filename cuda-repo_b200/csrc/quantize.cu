@@ -105,6 +105,9 @@ __global__ void __launch_bounds__(512, 2) quantize_strips_kernel(const uint16_t*
     __shared__ uint32_t tops[kMaxStripCtas][8];
     __shared__ RowScale rs[8];
     const int ctas = (int)ptx::cluster_nctarank(), rank = (int)ptx::cluster_ctarank();
+    // "This CTA runs", awaited before the first store into another's shared
+    // memory: the loads pass meanwhile.
+    if (ctas > 1) ptx::cluster_arrive_release();
     ptx::grid_dep_wait();
     if (threadIdx.x == 0) ptx::grid_dep_launch();
     const int strip_id = (int)blockIdx.x / ctas, row0 = strip_id * 8;
@@ -135,6 +138,7 @@ __global__ void __launch_bounds__(512, 2) quantize_strips_kernel(const uint16_t*
         }
     }
     __syncthreads();
+    if (ctas > 1) ptx::cluster_wait_acquire();  // every CTA of the cluster runs
     if ((int)threadIdx.x < 8 * ctas) {  // this CTA's maxima into every CTA's slot of it
         const int j = threadIdx.x & 7, to = threadIdx.x >> 3;
         uint32_t t = 0u;
