@@ -183,6 +183,22 @@ __device__ __forceinline__ float moe_activate(float y, int act) {
     return y;
 }
 
+// int8: h -> rint(127 h / a), ties to even, exactly, for fp32 |h| <= a; inv =
+// RN(127 / a).  The product h inv is off by its own rounding and inv's, each
+// 2^-24 of at most 127: less than 2^-16 together.  So it names the integer unless it
+// lies that near to a tie k + 1/2 (one value in 2^14); there 254 |h| against (2k + 1) a
+// decides, products of 24 and 8 bits that doubles hold.
+__device__ __forceinline__ uint32_t moe_round_h(float h, float a, float inv) {
+    const float p = fabsf(h) * inv;
+    float q = rintf(p);
+    if (fabsf(fabsf(p - q) - 0.5f) < 0x1p-15f) {
+        const float k = floorf(p);
+        const double d = 254.0 * (double)fabsf(h) - (2.0 * (double)k + 1.0) * (double)a;
+        q = d > 0.0 || (d == 0.0 && ((int)k & 1)) ? k + 1.f : k;
+    }
+    return (uint32_t)(int)copysignf(q, h);
+}
+
 // ------------------------------------------------------------------ router
 // Unit (expert, strip of eight tokens, K share): a block, eight partial
 // logits.  A lane takes eight consecutive inputs at a time.  Shares of about
@@ -1100,13 +1116,14 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
 #pragma unroll
                     for (int n = 0; n < AHEAD; ++n) {
                         if (a[n] == -1.f) continue;
-                        const float inv = 127.f / a[n];
-                        // else the row is zero (or below 1e-36), infinite or NaN: zeros, times its scale
-                        const bool finite = inv > 0.f && inv <= 3.402823466e38f;
+                        // a row of zeros, or one with an infinity or NaN: zeros, times its scale
+                        const bool live = a[n] > 0.f && a[n] <= 3.402823466e38f;
+                        // far below 1, 127 / a would overflow: both times 2^64, which changes no quotient
+                        const float pre = a[n] < 0x1p-60f ? 0x1p64f : 1.f, top = a[n] * pre, inv = 127.f / top;
                         const float hv[4] = {h[n].x, h[n].y, h[n].z, h[n].w};
                         uint32_t q[4];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) q[i] = finite ? (uint32_t)__float2int_rn(hv[i] * inv) : 0u;
+                        for (int i = 0; i < 4; ++i) q[i] = live ? moe_round_h(hv[i] * pre, top, inv) : 0u;
                         *reinterpret_cast<uint32_t*>(p.hq + at[n]) = pack4(q[0], q[1], q[2], q[3]);
                     }
                 }

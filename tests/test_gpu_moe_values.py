@@ -1,0 +1,95 @@
+"""spmm24_launch_moe where its values are delicate: rows of h next to ties,
+rows of tiny values."""
+import numpy as np
+import pytest
+
+import spmm24
+from test_gpu_moe import _strips
+
+pytestmark = pytest.mark.gpu
+
+
+def _round_exactly(h, a):
+    """rint(127 h / a), ties to even, of integers."""
+    n, d = 127 * np.abs(h), a
+    q, r = n // d, n % d
+    q = q + ((2 * r > d) | ((2 * r == d) & (q % 2 == 1)))
+    return np.sign(h) * q
+
+
+def _hard_rows(count, seed):
+    """Rows of 128 integers, the first the largest: values on a tie or next to one, those first that a product with
+    the rounded quotient 127 / a takes to the wrong side."""
+    rng = np.random.default_rng(seed)
+    rows = []
+    while len(rows) < count:
+        a = int(rng.integers(100000, 400000))
+        if len(rows) % 2:
+            a = 254 * (a // 508 * 2 + 1)  # (2k + 1) a / 254 is an integer: exact ties
+            a = a if a < 400000 else a - 254 * 400
+        k = np.arange(127)
+        h = np.concatenate([(2 * k + 1) * a // 254 + d for d in (0, 1)])
+        h = np.concatenate([h, -h])
+        h = h[(np.abs(h) <= a)]
+        fast = np.rint(h.astype(np.float32) * (np.float32(127) / np.float32(a)))
+        wrong = fast != _round_exactly(h, a)
+        order = np.argsort(~wrong, kind="stable")
+        rows.append(np.concatenate([[a], h[order][:127]]))
+    rows = np.array(rows)
+    fast = np.rint(rows.astype(np.float32) * (np.float32(127) / rows[:, :1].astype(np.float32)))
+    assert (fast != _round_exactly(rows, rows[:, :1])).any()  # hard ones are among them
+    return rows
+
+
+def _integer_layer(device, rows, unit, d_scale):
+    """T tokens, each with an expert of its own whose h is the integers `rows` times unit ** 2: gate rows that sum
+    to them, up rows that pick a one, the identity for down."""
+    import torch
+
+    T, H = rows.shape[0], 128
+    x = np.full(H, 127, dtype=np.float32)  # scale 1
+    x[4] = 1
+    gu = np.zeros((T, 2 * H, H), dtype=np.int8)
+    for e in range(T):
+        for i, v in enumerate(rows[e]):
+            tens = int(np.round(v / 127))
+            gu[e, i, 4] = v - 127 * tens
+            for k in list(range(8, 128, 4)) + list(range(9, 128, 4)):  # at most two of each four
+                w = int(np.clip(tens, -127, 127))
+                gu[e, i, k] = w
+                tens -= w
+            assert tens == 0 and abs(v) < 127 * 127 * 60
+            gu[e, H + i, 4] = 1
+        assert np.array_equal(gu[e].astype(np.int64) @ x.astype(np.int64), np.concatenate([rows[e], np.ones(H, np.int64)]))
+    eye = np.tile(np.eye(H, dtype=np.int8), (T, 1))
+    up = lambda m: [torch.from_numpy(v).to(device) for v in spmm24.compress_a_int8(m, m.shape[0], H)]  # noqa: E731
+    return (torch.from_numpy(x).to(device).expand(T, H), up(gu.reshape(-1, H)), up(eye),
+            torch.full((T * 2 * H,), unit, device=device), torch.full((T * H,), d_scale, device=device))
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("unit,d_scale", [(1.0, 1.0), (2.0 ** -70, 2.0 ** 120)], ids=["ones", "tiny"])
+def test_rows_of_h_round_exactly(cuda_device, unit, d_scale, bf16):
+    """Ties, their neighbours, and rows whose largest value is near the end of fp32's range (where 127 / max
+    overflows): every int8 value of h is what the formula gives."""
+    import torch
+
+    T, H = 32, 128
+    rows = _hard_rows(T, 1)
+    dt = torch.bfloat16 if bf16 else torch.float16
+    x, gu, dn, gs, ds = _integer_layer(cuda_device, rows, unit, d_scale)
+    flags = spmm24.MOE_INT8 | (spmm24.BF16 if bf16 else 0)
+    ws = torch.zeros(spmm24.moe_workspace_bytes(T, H, H, T, 1, flags), dtype=torch.uint8, device=cuda_device)
+    ids = torch.arange(T, dtype=torch.int32, device=cuda_device).reshape(T, 1)
+    w = 2.0 ** -8
+    weights = torch.full((T, 1), w, device=cuda_device)
+    y = torch.zeros(H, T, dtype=dt, device=cuda_device)
+    rc = spmm24.launch_moe(torch.cuda.current_stream(cuda_device), _strips(x.to(dt)), None, gu[0], gu[1], dn[0], dn[1], y, T, H,
+                           H, T, 1, ws, flags=flags, gate_up_scale=gs, down_scale=ds, topk_ids=ids, topk_weights=weights,
+                           activation=spmm24.ACT_NONE)
+    assert rc == 0, spmm24._lib.spmm24_last_error().decode()
+    a = rows[:, 0].astype(np.float64) * unit * unit
+    # y = w a / 127 d q, off by 2^-8 of 127 at most and a few fp32 steps (2^-20 for a / 127 next to fp32's smallest): below 1/2
+    q = y.double().cpu().numpy().T / (w * a / 127 * d_scale)[:, None]
+    assert np.array_equal(np.rint(q).astype(np.int64), _round_exactly(rows, rows[:, :1]))
+    assert spmm24.device_status(0) == 0
