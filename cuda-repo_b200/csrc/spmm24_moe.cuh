@@ -174,13 +174,19 @@ struct MoeRuns {
     }
 };
 
-// SiLU and GELU (tanh form, as y sigmoid(2 z)) to fp32 accuracy: the few
-// values of this layer are no load, and h is rounded after them.
+// SiLU y sigmoid(y), and GELU's tanh form 0.5 y (1 + tanh z) as y sigmoid(2 z),
+// to a few steps of fp32 beside the value itself: y / (1 + e^-x), and y e^x where x is so
+// low that e^-x could overflow (1 + e^x is 1 there).  expf and the division are
+// the exact kinds: the few values of this layer are no load, and h, which is rounded
+// next, takes another value wherever it crosses a border.  GELU's x has seven
+// roundings of its own (2^-24 each), which e^-x sees |x| times.
 __device__ __forceinline__ float moe_activate(float y, int act) {
     if (act == kActRelu) return y > 0.f || y != y ? y : 0.f;
-    if (act == kActSilu) return __fdividef(y, 1.f + __expf(-y));
-    if (act == kActGelu) return __fdividef(y, 1.f + __expf(-1.5957691216057308f * (y + 0.044715f * y * y * y)));
-    return y;
+    if (act != kActSilu && act != kActGelu) return y;
+    const float x = act == kActSilu ? y : 1.5957691216057308f * (y + 0.044715f * y * y * y);
+    const bool low = x < -80.f;
+    const float e = expf(low ? x : -x);
+    return low ? y * e : y / (1.f + e);
 }
 
 // int8: h -> rint(127 h / a), ties to even, exactly, for fp32 |h| <= a; inv =
@@ -1004,10 +1010,12 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
                             const int t = 8 * s + 2 * q;
-                            w[q] = pack2(
-                                moe_activate(__uint_as_float(v[t]), p.act) * __uint_as_float(v[N_TILE + t]),
-                                moe_activate(__uint_as_float(v[t + 1]), p.act) * __uint_as_float(v[N_TILE + t + 1]),
-                                p.bf16);
+                            w[q] = 0u;  // a pair of tokens that have other experts
+                            if (mask >> t & 3u)
+                                w[q] = pack2(
+                                    moe_activate(__uint_as_float(v[t]), p.act) * __uint_as_float(v[N_TILE + t]),
+                                    moe_activate(__uint_as_float(v[t + 1]), p.act) * __uint_as_float(v[N_TILE + t + 1]),
+                                    p.bf16);
                         }
                         *reinterpret_cast<uint4*>(p.h16 + (((size_t)slot * p.strips + s) * p.I + r) * 8) =
                             make_uint4(w[0], w[1], w[2], w[3]);

@@ -1,9 +1,10 @@
 """spmm24_launch_moe where its values are delicate: rows of h next to ties,
-rows of tiny values."""
+rows of tiny values, gates far below zero."""
 import numpy as np
 import pytest
 
 import spmm24
+from act_values import act_tails
 from test_gpu_moe import _strips
 
 pytestmark = pytest.mark.gpu
@@ -93,3 +94,38 @@ def test_rows_of_h_round_exactly(cuda_device, unit, d_scale, bf16):
     q = y.double().cpu().numpy().T / (w * a / 127 * d_scale)[:, None]
     assert np.array_equal(np.rint(q).astype(np.int64), _round_exactly(rows, rows[:, :1]))
     assert spmm24.device_status(0) == 0
+
+
+@pytest.mark.parametrize("act", [2, 3], ids=["silu", "gelu"])
+def test_gates_far_below_zero(cuda_device, act):
+    """Gates down to where e^-gate overflows fp32, times an up value of 2^100 that makes the smallest products
+    ordinary numbers: h is held to the activation's own size.
+
+    Bound, relative: expf, 1 + e, the quotient, the products: 10 steps of 2^-23, and 16 more where e^x is below 2^-126
+    (four bits are lost at e^-90); GELU's exponent is off by seven roundings of 2^-24, which e^x sees |x| times.  h and y
+    round to bf16 once each."""
+    import torch
+
+    H = 128
+    gates = np.linspace(-90, 8, H) if act == 2 else np.linspace(-10.1, 8, H)
+    w = torch.zeros(2 * H, H, dtype=torch.bfloat16, device=cuda_device)
+    w[:H, 0] = torch.from_numpy(gates).to(cuda_device).bfloat16()
+    w[H:, 0] = 2.0 ** 100
+    gate = w[:H, 0].double()
+    x = torch.zeros(1, H, dtype=torch.bfloat16, device=cuda_device)
+    x[0, 0] = 1
+    gu = spmm24.pack_a_device(w, 2 * H, H)[:2]
+    dn = spmm24.pack_a_device(torch.eye(H, dtype=torch.bfloat16, device=cuda_device), H, H)[:2]
+    ws = torch.zeros(spmm24.moe_workspace_bytes(1, H, H, 1, 1, spmm24.BF16), dtype=torch.uint8, device=cuda_device)
+    ids = torch.zeros(1, 1, dtype=torch.int32, device=cuda_device)
+    y = torch.zeros(H, 1, dtype=torch.bfloat16, device=cuda_device)
+    rc = spmm24.launch_moe(torch.cuda.current_stream(cuda_device), _strips(x), None, gu[0], gu[1], dn[0], dn[1], y, 1, H, H, 1, 1,
+                           ws, flags=spmm24.BF16, topk_ids=ids, topk_weights=torch.ones(1, 1, device=cuda_device),
+                           activation=act)
+    assert rc == 0, spmm24._lib.spmm24_last_error().decode()
+    ref, size = act_tails(gate, act)
+    ref = ref * 2.0 ** 100
+    rel = (26 + (0 if act == 2 else 3.5) * size) * 2.0 ** -23
+    off = (y[:, 0].double() - ref).abs()
+    tol = ref.abs() * (rel + 2 * 2.0 ** -8)
+    assert (off <= tol).all(), float((off / tol).max())
