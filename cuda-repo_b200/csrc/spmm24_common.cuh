@@ -345,7 +345,9 @@ __device__ __forceinline__ bool epilogue_is_plain(const Epilogue& e) {
 // alpha, bias and activation on n values of row gm (no residual).
 // bias_pre: the row's bias already loaded (e.g. prefetched into shared
 // memory while the main loop ran), or null to read e.bias[gm].
-template <int n>
+// KEEP: a ReLU that keeps NaN, by which the int8 products and the expert layer
+// mark a token that holds no number (fmaxf makes it 0).
+template <int n, bool KEEP = false>
 __device__ __forceinline__ void epilogue_pre(float* y, const Epilogue& e, int gm, const float* bias_pre = nullptr) {
     if (e.alpha != 1.f) {
 #pragma unroll
@@ -358,7 +360,7 @@ __device__ __forceinline__ void epilogue_pre(float* y, const Epilogue& e, int gm
     }
     if (e.act == kActRelu) {
 #pragma unroll
-        for (int i = 0; i < n; ++i) y[i] = fmaxf(y[i], 0.f);
+        for (int i = 0; i < n; ++i) y[i] = KEEP ? (y[i] <= 0.f ? 0.f : y[i]) : fmaxf(y[i], 0.f);
     } else if (e.act == kActSilu) {
 #pragma unroll
         for (int i = 0; i < n; ++i) y[i] = activate(y[i], kActSilu);
@@ -382,6 +384,7 @@ __device__ __forceinline__ void round8(const float* y, int lim, int bf16, uint32
 // uniform branch, so an unused stage costs nothing.
 // res_pre: the 8 residual values already loaded (16-byte layouts only), or
 // null to read them from e.residual.
+template <bool KEEP>
 __device__ __forceinline__ void epilogue8(const float* v, const Epilogue& e, int gm, int gn, int M, int N,
                                           bool vec_rowmajor, uint32_t* w, const float* bias_pre = nullptr,
                                           const uint4* res_pre = nullptr) {
@@ -389,7 +392,7 @@ __device__ __forceinline__ void epilogue8(const float* v, const Epilogue& e, int
     float y[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] = v[i];
-    epilogue_pre<8>(y, e, gm, bias_pre);
+    epilogue_pre<8, KEEP>(y, e, gm, bias_pre);
     if (e.residual) {
         const size_t base = c_offset(e, gm, gn, M, N);
         if (e.packed || vec_rowmajor) {
@@ -407,13 +410,14 @@ __device__ __forceinline__ void epilogue8(const float* v, const Epilogue& e, int
 // Epilogue + the store into C of 8 columns of row gm < M (gn < N).  A packed
 // C is always written as whole 16-byte strip rows.  `plain`: the caller's
 // epilogue_is_plain(e), evaluated once per kernel.
+template <bool KEEP = false>
 __device__ __forceinline__ void epilogue_store8(uint16_t* C, const float* v, const Epilogue& e, int gm, int gn, int M,
                                                 int N, bool vec_rowmajor, bool plain, const float* bias_pre = nullptr,
                                                 const uint4* res_pre = nullptr) {
     const int lim = min(8, N - gn);
     uint32_t w[4];
     if (plain) round8(v, lim, e.bf16, w);
-    else epilogue8(v, e, gm, gn, M, N, vec_rowmajor, w, bias_pre, res_pre);
+    else epilogue8<KEEP>(v, e, gm, gn, M, N, vec_rowmajor, w, bias_pre, res_pre);
     if (e.packed) {
         *reinterpret_cast<uint4*>(C + c_offset(e, gm, gn, M, N)) = make_uint4(w[0], w[1], w[2], w[3]);
     } else if (vec_rowmajor) {

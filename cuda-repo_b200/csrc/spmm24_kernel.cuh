@@ -413,7 +413,7 @@ spmm24_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
             const int gn = n0 + ch * 8;
             if (gm >= p.M || gn >= p.N) continue;
             if constexpr (EPI) {
-                epilogue_store8(p.C, acc, p.epi, gm, gn, p.M, p.N, vec_ok, epilogue_is_plain(p.epi),
+                epilogue_store8<I8>(p.C, acc, p.epi, gm, gn, p.M, p.N, vec_ok, epilogue_is_plain(p.epi),
                                 p.epi.bias ? bias_s + lr : nullptr, res_pre ? res_s + lr * CHUNKS + ch : nullptr);
             } else {
                 if constexpr (FP8) {
@@ -877,7 +877,7 @@ spmm24_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
                         f[e] = I8 ? int8_value((int)v[e], wsc, xscale_s[c * 16 + e]) : __uint_as_float(v[e]);
-                    if (gm < p.M) epilogue_pre<16>(f, p.epi, gm);
+                    if (gm < p.M) epilogue_pre<16, I8>(f, p.epi, gm);
                     float4* dst = reinterpret_cast<float4*>(fst + (size_t)row * C_::F_PITCH + c * 16);
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
@@ -894,7 +894,7 @@ spmm24_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
                         f[e] = I8 ? int8_value((int)v[e], wsc, xscale_s[c * 16 + e]) : __uint_as_float(v[e]);
-                    if (gm < p.M) epilogue_pre<16>(f, p.epi, gm);
+                    if (gm < p.M) epilogue_pre<16, I8>(f, p.epi, gm);
                     const int gn = gn0 + c * 16;
                     uint32_t h[8];
                     if (gn + 16 <= p.N) {
@@ -1281,7 +1281,7 @@ spmm24_pair2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
                         y[e] = I8 ? int8_value((int)v[e], wsc, xscale_s[c * 16 + e]) : __uint_as_float(v[e]);
-                    if (gmh < p.M) epilogue_pre<16>(y, p.epi, gmh);
+                    if (gmh < p.M) epilogue_pre<16, I8>(y, p.epi, gmh);
                     uint32_t w[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) w[e] = pack2(y[2 * e], y[2 * e + 1], p.epi.bf16);

@@ -1154,7 +1154,7 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
                 float f[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(y[c + i]);
-                epilogue_store8(p.y, f, p.epi, gm, c, p.H, p.T, vec, plain);
+                epilogue_store8<true>(p.y, f, p.epi, gm, c, p.H, p.T, vec, plain);
             }
         };
         uint64_t* const part2 = p.part + (size_t)kMoeMaxCtas * 2 * kMoeSlotWords;  // the first group's down partials
@@ -1240,7 +1240,7 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
                         float y[8];
 #pragma unroll
                         for (int i = 0; i < 8; ++i) y[i] = __uint_as_float(v[i]);
-                        epilogue_store8(p.y, y, p.epi, gm, t0, p.H, p.T, vec, plain);
+                        epilogue_store8<true>(p.y, y, p.epi, gm, t0, p.H, p.T, vec, plain);
                     } else {
 #pragma unroll
                         for (int i = 0; i < 2 * PAIRS; ++i) {
@@ -1249,7 +1249,7 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
                             const size_t at = c_offset(p.epi, gm, tok, p.H, p.T);
                             float y[1] = {__uint_as_float(v[i])};
                             if (!plain) {
-                                epilogue_pre<1>(y, p.epi, gm);
+                                epilogue_pre<1, true>(y, p.epi, gm);
                                 if (p.epi.residual && tok < p.T) y[0] += elem_to_f32(p.epi.residual[at], p.epi.bf16);
                             }
                             p.y[at] = tok < p.T ? f32_to_elem(y[0], p.epi.bf16) : (uint16_t)0;

@@ -262,7 +262,7 @@ spmm24_prefill_int8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
                     float y[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) y[e] = int8_value((int)v[8 * q + e], wsc, s[e]);
-                    epilogue_pre<8>(y, p.epi, gm, &b);
+                    epilogue_pre<8, true>(y, p.epi, gm, &b);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) o[e] = pack2(y[2 * e], y[2 * e + 1], p.epi.bf16);
                 };

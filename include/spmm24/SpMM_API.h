@@ -381,7 +381,9 @@ cudaError_t spmm24_launch_fp8(cudaStream_t stream, const void* values, const voi
  * Values, metadata and B have the fp8 extension's layouts (K % 128 == 0,
  * M % 16 == 0, K < 262144), bytes being int8; a weight of -128 is allowed, and
  * only the byte 0 is a zero.  The sum being exact, every split_k gives the
- * same bits.  C, bias and residual are fp16 (bf16 with SPMM24_BF16). */
+ * same bits.  C, bias and residual are fp16 (bf16 with SPMM24_BF16).  A NaN
+ * stays NaN through every activation (the ReLU of the other launches makes it
+ * 0), so that a token whose scale is no number can be told by its column. */
 
 /* 16-bit rows -> int8 rows and one scale for each row: activations (a row =
  * a token) or weights (a row = an output channel).
@@ -432,7 +434,8 @@ cudaError_t spmm24_launch_int8(cudaStream_t stream, const void* values, const vo
  * (fp16; bf16 with SPMM24_BF16): h is rounded to the operand type.  int8
  * experts (SPMM24_MOE_INT8): x_t is rounded to int8 as spmm24_quantize_int8
  * rounds rows, every h likewise (scale max |h| / 127), sums are exact and
- * scaled by channel and row; x, router and y stay 16-bit.
+ * scaled by channel and row; x, router and y stay 16-bit.  A NaN stays NaN
+ * through every activation, the gate's and the epilogue's.
  * The result does not depend on timing: the same call gives the same bits.
  *
  *   tokens      1..32 (T); hidden H and inter I: multiples of 64 (int8: 128);

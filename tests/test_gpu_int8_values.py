@@ -1,10 +1,10 @@
 """The int8 quantiser and product where their values are delicate: clusters
-that wait for room, tokens that hold no number, activations far below zero."""
+that wait for room, tokens that hold no number."""
 import numpy as np
 import pytest
 
 import spmm24
-from int8_problems import bits_to_f64
+from int8_problems import bits_to_f64, problem
 from test_gpu_int8 import _dev, _quantized, _random_bits
 
 pytestmark = pytest.mark.gpu
@@ -32,3 +32,46 @@ def test_strips_beside_other_work(cuda_device):
     torch.cuda.synchronize(cuda_device)
     for q, s in outs:
         assert torch.equal(q, want_q) and torch.equal(s, want_s)
+
+
+# every kernel of the product, and a shape that it takes
+KERNELS = {"cluster": (dict(pair=0), 528, 269, 256), "cluster16": (dict(pair=0, tile_n=16), 528, 40, 256),
+           "pair": (dict(pair=1, pair2=0, pair_split=1), 528, 269, 256),
+           "pair-split": (dict(pair=1, pair2=0, pair_split=2), 528, 269, 512),
+           "pair2": (dict(pair=1, pair2=1), 1040, 269, 256), "persistent": (dict(pair2=1), 5120, 2048, 256)}
+
+
+def _product(device, M, N, K, seed):
+    """(values, metadata, B, exact sums) of a problem on the device."""
+    import torch
+
+    a, b = problem(M, N, K, seed)
+    vals, meta = spmm24.compress_a_int8(a, M, K)
+    acc = torch.from_numpy(a).to(device).double() @ torch.from_numpy(b).to(device).double().T
+    return _dev(vals, device), _dev(meta, device), _dev(b, device), acc
+
+
+@pytest.mark.parametrize("act", [0, 1, 2, 3], ids=["none", "relu", "silu", "gelu"])
+@pytest.mark.parametrize("kernel", list(KERNELS))
+@pytest.mark.parametrize("packed", [False, True], ids=["rows", "strips"])
+def test_a_token_that_holds_no_number_stays_so(cuda_device, tuning, kernel, act, packed):
+    """Infinite and NaN scales (the quantiser's for such rows): their columns are NaN, whatever the activation."""
+    import torch
+
+    kw, M, N, K = KERNELS[kernel]
+    tuning(**kw)
+    vals, meta, b, _ = _product(cuda_device, M, N, K, 3)
+    bad = [0, 7, 21, N - 1]
+    scale = torch.full((N,), 2.0 ** -13, device=cuda_device)
+    scale[bad] = torch.tensor([float("nan"), float("inf"), float("nan"), float("inf")], device=cuda_device)
+    b = b.clone()
+    b[bad] = 0  # as the quantiser writes them: 0 * inf
+    strips = (N + 7) // 8
+    c = torch.zeros(strips * 8 * M, dtype=torch.float16, device=cuda_device)
+    bias = torch.ones(M, dtype=torch.float16, device=cuda_device)
+    rc = spmm24.launch_int8(torch.cuda.current_stream(cuda_device), vals, b, meta, c, M, N, K, x_scale=scale, bias=bias,
+                            activation=act, out_layout=spmm24.OUT_PACKED_B if packed else spmm24.OUT_ROW_MAJOR)
+    assert rc == 0
+    y = c.reshape(strips, M, 8).transpose(0, 1).reshape(M, -1)[:, :N] if packed else c[: M * N].reshape(M, N)
+    nan = torch.isnan(y)
+    assert nan[:, bad].all() and int(nan.sum()) == M * len(bad)

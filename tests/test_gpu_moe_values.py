@@ -1,11 +1,12 @@
 """spmm24_launch_moe where its values are delicate: rows of h next to ties,
-rows of tiny values, gates far below zero."""
+rows of tiny values, gates far below zero, epilogues of tokens that hold no
+number."""
 import numpy as np
 import pytest
 
 import spmm24
 from act_values import act_tails
-from test_gpu_moe import _strips
+from test_gpu_moe import Layer, _strips
 
 pytestmark = pytest.mark.gpu
 
@@ -128,4 +129,45 @@ def test_gates_far_below_zero(cuda_device, act):
     rel = (26 + (0 if act == 2 else 3.5) * size) * 2.0 ** -23
     off = (y[:, 0].double() - ref).abs()
     tol = ref.abs() * (rel + 2 * 2.0 ** -8)
+    assert (off <= tol).all(), float((off / tol).max())
+
+
+@pytest.mark.parametrize("act", [1], ids=["relu"])
+@pytest.mark.parametrize("T", [3, 16, 20], ids=lambda t: "T%d" % t)
+@pytest.mark.parametrize("int8", [False, True], ids=["fp16", "int8"])
+def test_epilogue_activations(cuda_device, act, T, int8):
+    """An activation of y: tokens with an infinity or NaN keep it, and values far below zero are right beside their
+    own size (one expert of weight 1; alpha makes most of y lie in -12 .. 12)."""
+    import torch
+
+    L = Layer(cuda_device, 256, 384, 4, int8=int8, seed=act)
+    x = L.tokens(T)
+    x[1, 5] = float("nan")
+    x[2, 9] = float("inf")
+    ids = torch.randint(0, 4, (T, 1), generator=L.g, device=cuda_device, dtype=torch.int32)
+    w = torch.ones(T, 1, device=cuda_device)
+    ws = L.workspace(T, 1)
+    pre, _, _ = L.run(x, 1, ws, ids=ids, weights=w)
+    scale = 2.0 ** float(torch.log2(4 / L.result(pre, T)[:, 3 if T > 3 else 0].std()).round())
+    bias = torch.zeros(256, dtype=torch.float16, device=cuda_device)
+    bias[::2] = -6
+    out, _, _ = L.run(x, 1, ws, ids=ids, weights=w, alpha=scale, bias=bias, epilogue_activation=act)
+    got = L.result(out, T)
+    assert torch.isnan(got[:, 1]).all() and not torch.isfinite(got[:, 2]).any()
+    keep = [t for t in range(T) if t not in (1, 2)]
+    # y before the activation, to 16 bits, from the layer itself; the activated one must come of a value that rounds to it
+    lin, _, _ = L.run(x, 1, ws, ids=ids, weights=w, alpha=scale, bias=bias)
+    lin = L.result(lin, T)[:, keep]
+    got = got[:, keep]
+    assert (lin < -7).any() and (lin > 0).any()
+    step = 2.0 ** -11 * lin.abs() + 2.0 ** -25
+    if act == 1:
+        assert torch.equal(got, lin.clamp(min=0))
+        return
+    ref, size = act_tails(lin, act)
+    lo, hi = act_tails(lin - step, act)[0], act_tails(lin + step, act)[0]
+    spread = (lo - ref).abs().maximum((hi - ref).abs())
+    rel = (5 + 4.7 * size.clamp(max=110)) * 2.0 ** -23
+    off = (got - ref).abs()
+    tol = spread + (ref.abs() + spread) * (2.0 ** -11 + 2 * rel) + 2.0 ** -25
     assert (off <= tol).all(), float((off / tol).max())
