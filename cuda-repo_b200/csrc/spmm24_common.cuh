@@ -303,8 +303,7 @@ __device__ __forceinline__ float int8_value(int acc, float w_scale, float x_scal
     return (float)acc * w_scale * x_scale;
 }
 
-// Hardware tanh approximation (tanh.approx.f32: relative error about 2^-11,
-// far below an fp16 / bf16 output ulp).
+// Hardware tanh approximation (tanh.approx.f32: relative error about 2^-11).
 __device__ __forceinline__ float tanh_fast(float x) {
     float y;
     asm("tanh.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -313,12 +312,34 @@ __device__ __forceinline__ float tanh_fast(float x) {
 
 // ReLU; SiLU y * sigmoid(y), with sigmoid(y) = 0.5 + 0.5 tanh(y / 2); GELU
 // in its tanh form (Hendrycks & Gimpel, 2016): 0.5 y (1 + tanh(sqrt(2 / pi)
-// (y + 0.044715 y^3))).  One hardware tanh per element.
+// (y + 0.044715 y^3))).  One hardware tanh per element: the activations of the
+// 16-bit and fp8 launches.  Its error moves the result by up to 2^-12 |y|, half a step
+// of fp16 and a sixteenth of bf16's while y is positive; below zero, where the result
+// is small beside y, by more than that (all of it at SiLU(-9)).
 __device__ __forceinline__ float activate(float y, int act) {
     if (act == kActRelu) return fmaxf(y, 0.f);
     if (act == kActSilu) return y * fmaf(0.5f, tanh_fast(0.5f * y), 0.5f);
     if (act == kActGelu) return 0.5f * y * (1.f + tanh_fast(0.7978845608028654f * (y + 0.044715f * y * y * y)));
     return y;
+}
+
+// The activations of the int8 launches and the expert layer's epilogue.  A NaN
+// stays (it marks a token that holds no number; fmaxf would make it 0).  SiLU
+// y sigmoid(x), x = y, and GELU's tanh form with x = 2 sqrt(2 / pi) (y + 0.044715 y^3),
+// are right beside their own size: with t = e^-|x|, sigmoid(x) is 1 / (1 + t) or
+// t / (1 + t), where nothing cancels or overflows.  __expf is off by 2 + 1.17 |x| steps
+// of 2^-23 and __fdividef by two (GELU's x has roundings of its own, 3.5 |x| steps):
+// below 2^-13 of the result wherever it is a normal number of C's type.  Two special
+// functions an element, activate() has one: 11008 x 509 x 4096 with bias and SiLU, one
+// tile a pair with nothing to hide its epilogue behind, takes 30.2 us where that took
+// 28.5, all of it the second function's issue (a form with the bare exponential and
+// reciprocal instructions measured the same).
+__device__ __forceinline__ float activate_int8(float y, int act) {
+    if (act == kActRelu) return y <= 0.f ? 0.f : y;
+    if (act != kActSilu && act != kActGelu) return y;
+    const float x = act == kActSilu ? y : 1.5957691216057308f * (y + 0.044715f * y * y * y);
+    const float t = __expf(-fabsf(x));
+    return __fdividef(x < 0.f ? y * t : y, 1.f + t);
 }
 
 // Two values rounded to C's type, packed low-first in one word.
@@ -345,9 +366,8 @@ __device__ __forceinline__ bool epilogue_is_plain(const Epilogue& e) {
 // alpha, bias and activation on n values of row gm (no residual).
 // bias_pre: the row's bias already loaded (e.g. prefetched into shared
 // memory while the main loop ran), or null to read e.bias[gm].
-// KEEP: a ReLU that keeps NaN, by which the int8 products and the expert layer
-// mark a token that holds no number (fmaxf makes it 0).
-template <int n, bool KEEP = false>
+// I8: activate_int8 in place of activate.
+template <int n, bool I8 = false>
 __device__ __forceinline__ void epilogue_pre(float* y, const Epilogue& e, int gm, const float* bias_pre = nullptr) {
     if (e.alpha != 1.f) {
 #pragma unroll
@@ -360,13 +380,13 @@ __device__ __forceinline__ void epilogue_pre(float* y, const Epilogue& e, int gm
     }
     if (e.act == kActRelu) {
 #pragma unroll
-        for (int i = 0; i < n; ++i) y[i] = KEEP ? (y[i] <= 0.f ? 0.f : y[i]) : fmaxf(y[i], 0.f);
+        for (int i = 0; i < n; ++i) y[i] = I8 ? activate_int8(y[i], kActRelu) : fmaxf(y[i], 0.f);
     } else if (e.act == kActSilu) {
 #pragma unroll
-        for (int i = 0; i < n; ++i) y[i] = activate(y[i], kActSilu);
+        for (int i = 0; i < n; ++i) y[i] = I8 ? activate_int8(y[i], kActSilu) : activate(y[i], kActSilu);
     } else if (e.act == kActGelu) {
 #pragma unroll
-        for (int i = 0; i < n; ++i) y[i] = activate(y[i], kActGelu);
+        for (int i = 0; i < n; ++i) y[i] = I8 ? activate_int8(y[i], kActGelu) : activate(y[i], kActGelu);
     }
 }
 
@@ -384,7 +404,7 @@ __device__ __forceinline__ void round8(const float* y, int lim, int bf16, uint32
 // uniform branch, so an unused stage costs nothing.
 // res_pre: the 8 residual values already loaded (16-byte layouts only), or
 // null to read them from e.residual.
-template <bool KEEP>
+template <bool I8>
 __device__ __forceinline__ void epilogue8(const float* v, const Epilogue& e, int gm, int gn, int M, int N,
                                           bool vec_rowmajor, uint32_t* w, const float* bias_pre = nullptr,
                                           const uint4* res_pre = nullptr) {
@@ -392,7 +412,7 @@ __device__ __forceinline__ void epilogue8(const float* v, const Epilogue& e, int
     float y[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] = v[i];
-    epilogue_pre<8, KEEP>(y, e, gm, bias_pre);
+    epilogue_pre<8, I8>(y, e, gm, bias_pre);
     if (e.residual) {
         const size_t base = c_offset(e, gm, gn, M, N);
         if (e.packed || vec_rowmajor) {
@@ -410,14 +430,14 @@ __device__ __forceinline__ void epilogue8(const float* v, const Epilogue& e, int
 // Epilogue + the store into C of 8 columns of row gm < M (gn < N).  A packed
 // C is always written as whole 16-byte strip rows.  `plain`: the caller's
 // epilogue_is_plain(e), evaluated once per kernel.
-template <bool KEEP = false>
+template <bool I8 = false>
 __device__ __forceinline__ void epilogue_store8(uint16_t* C, const float* v, const Epilogue& e, int gm, int gn, int M,
                                                 int N, bool vec_rowmajor, bool plain, const float* bias_pre = nullptr,
                                                 const uint4* res_pre = nullptr) {
     const int lim = min(8, N - gn);
     uint32_t w[4];
     if (plain) round8(v, lim, e.bf16, w);
-    else epilogue8<KEEP>(v, e, gm, gn, M, N, vec_rowmajor, w, bias_pre, res_pre);
+    else epilogue8<I8>(v, e, gm, gn, M, N, vec_rowmajor, w, bias_pre, res_pre);
     if (e.packed) {
         *reinterpret_cast<uint4*>(C + c_offset(e, gm, gn, M, N)) = make_uint4(w[0], w[1], w[2], w[3]);
     } else if (vec_rowmajor) {

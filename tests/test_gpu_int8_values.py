@@ -1,9 +1,10 @@
 """The int8 quantiser and product where their values are delicate: clusters
-that wait for room, tokens that hold no number."""
+that wait for room, tokens that hold no number, activations far below zero."""
 import numpy as np
 import pytest
 
 import spmm24
+from act_values import act_tails
 from int8_problems import bits_to_f64, problem
 from test_gpu_int8 import _dev, _quantized, _random_bits
 
@@ -75,3 +76,34 @@ def test_a_token_that_holds_no_number_stays_so(cuda_device, tuning, kernel, act,
     y = c.reshape(strips, M, 8).transpose(0, 1).reshape(M, -1)[:, :N] if packed else c[: M * N].reshape(M, N)
     nan = torch.isnan(y)
     assert nan[:, bad].all() and int(nan.sum()) == M * len(bad)
+
+
+@pytest.mark.parametrize("act", [2, 3], ids=["silu", "gelu"])
+@pytest.mark.parametrize("bf16", [False, True], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("kernel", list(KERNELS))
+def test_activations_below_zero(cuda_device, tuning, kernel, bf16, act):
+    """Pre-activations within 100 of zero, most of them in -20 .. 20, exact in fp32 (powers of two for scales), against
+    the value itself: far below zero the activation is small, and its error has to be small beside it.
+
+    Bound, relative to the value: e^-x by the fast exponential 2 + 1.17 |x| steps of 2^-23, 1 + e half a one, the
+    fast division 2, the product with y half a one: (5 + 1.2 |x|) 2^-23.  GELU's x is itself the end of seven roundings
+    (two of them its constants) of 2^-24, which move e^-x by 3.5 |x| 2^-23.  Then half a step of C's type."""
+    import torch
+
+    kw, M, N, K = KERNELS[kernel]
+    tuning(**kw)
+    vals, meta, b, acc = _product(cuda_device, M, N, K, 5)
+    step = 2.0 ** -13 if K == 256 else 2.0 ** -14
+    c = torch.zeros(M, N, dtype=torch.bfloat16 if bf16 else torch.float16, device=cuda_device)
+    rc = spmm24.launch_int8(torch.cuda.current_stream(cuda_device), vals, b, meta, c, M, N, K, flags=spmm24.BF16 if bf16 else 0,
+                            x_scale=torch.full((N,), step, device=cuda_device), activation=act)
+    assert rc == 0
+    pre = acc * step
+    assert (pre < -8).any() and (pre > 8).any() and pre.abs().max() < 100
+    ref, x = act_tails(pre, act)
+    half, tiny = (2.0 ** -8, 2.0 ** -134) if bf16 else (2.0 ** -11, 2.0 ** -25)
+    # x is capped where the value is below every subnormal of C's type
+    rel = (5 + (1.2 if act == 2 else 4.7) * x.clamp(max=110)) * 2.0 ** -23
+    off = (c.double() - ref).abs()
+    tol = ref.abs() * (half + rel * (1 + half)) + tiny
+    assert (off <= tol).all(), float((off / tol).max())

@@ -132,7 +132,7 @@ def test_gates_far_below_zero(cuda_device, act):
     assert (off <= tol).all(), float((off / tol).max())
 
 
-@pytest.mark.parametrize("act", [1], ids=["relu"])
+@pytest.mark.parametrize("act", [1, 2, 3], ids=["relu", "silu", "gelu"])
 @pytest.mark.parametrize("T", [3, 16, 20], ids=lambda t: "T%d" % t)
 @pytest.mark.parametrize("int8", [False, True], ids=["fp16", "int8"])
 def test_epilogue_activations(cuda_device, act, T, int8):
