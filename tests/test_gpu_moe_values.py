@@ -1,6 +1,6 @@
 """spmm24_launch_moe where its values are delicate: rows of h next to ties,
 rows of tiny values, gates far below zero, epilogues of tokens that hold no
-number."""
+number, and 17 to 32 tokens with the experts in two groups."""
 import numpy as np
 import pytest
 
@@ -171,3 +171,45 @@ def test_epilogue_activations(cuda_device, act, T, int8):
     off = (got - ref).abs()
     tol = spread + (ref.abs() + spread) * (2.0 ** -11 + 2 * rel) + 2.0 ** -25
     assert (off <= tol).all(), float((off / tol).max())
+
+
+# hidden x inter so that gate / up has eight units or more for each CTA, and down a tile or less
+TWO_GROUPS = [(17, 2048, 1152, 20, 4), (32, 4096, 1408, 8, 2), (19, 3200, 1408, 9, 3), (31, 2176, 2816, 16, 2)]
+
+
+@pytest.mark.parametrize("shape", TWO_GROUPS, ids=lambda s: "T%d-%dx%d-E%dk%d" % s)
+@pytest.mark.parametrize("kind", ["fp16", "bf16", "int8-fp16", "int8-bf16"])
+def test_many_tokens_in_two_groups(cuda_device, shape, kind):
+    import torch
+
+    T, H, inter, E, k = shape
+    int8 = kind.startswith("int8")
+    L = Layer(cuda_device, H, inter, E, bf16=kind.endswith("bf16"), int8=int8, seed=T + E)
+    x = L.tokens(T)
+    ids, w, w_err = L.routed(x, k, True)
+    sms = torch.cuda.get_device_properties(cuda_device).multi_processor_count
+    stages = (H // (128 if int8 else 64) + 1) // 2
+    assert len(ids.unique()) * -(-inter // 128) * stages >= 8 * sms and -(-H // 128) <= sms  # two groups
+    ws = L.workspace(T, k)
+    out, got_ids, got_w = L.run(x, k, ws)
+    got = L.result(out, T)
+    assert torch.equal(got_ids.long(), ids) and ((got_w.double() - w).abs() <= w_err * w).all()
+    L.check(got, *L.reference(x, ids, w, w_err=w_err))
+    for _ in range(5):  # on a workspace that was used, the same bits
+        again, _, _ = L.run(x, k, ws)
+        torch.cuda.synchronize()
+        assert torch.equal(again, out)
+    # another routing on the same workspace: tokens without an expert, one named twice, a packed y with a residual
+    ids2 = ids.flip(0).to(torch.int32).contiguous()
+    ids2[0] = -1
+    ids2[1] = ids2[1, 0]
+    w2 = torch.randn(T, k, generator=L.g, device=cuda_device)
+    n = (T + 7) // 8 * 8 * H
+    res = torch.zeros((T + 7) // 8 * 8, H, dtype=L.dt, device=cuda_device)
+    res[:T] = torch.randn(T, H, generator=L.g, device=cuda_device).to(L.dt)
+    y = torch.full((n + 64,), 777.0, dtype=L.dt, device=cuda_device)
+    y[:n] = res.reshape(-1, 8, H).transpose(1, 2).reshape(-1)
+    out, _, _ = L.run(x, k, ws, ids=ids2, weights=w2, y=y, residual=y, packed=True)
+    ref, bound = L.reference(x, ids2.long(), w2)
+    r = res[:T].T.double()
+    L.check(L.result(out, T, True), ref + r, bound + 2.0 ** -22 * (ref.abs() + r.abs()))
