@@ -1419,6 +1419,7 @@ cudaError_t launch_moe_impl(cudaStream_t stream, const spmm24_moe_layer* L, unsi
         !act_map(&mp.tmH, i8 ? (const void*)mp.hq : (const void*)mp.h16, I, lay.slots))
         return invalid("moe: a TMA descriptor could not be encoded");
     const int ctas = moe_ctas(sm_count(dev));
+    if (i8 && lay.slots > (kMoeRunExperts - 1) * ctas) return invalid("moe int8: too few SMs for so many experts");
     if (i8)
         return n_tile == 16 ? launch_moe_kernel<16, true>(stream, dev, ctas, mp)
                             : launch_moe_kernel<32, true>(stream, dev, ctas, mp);

@@ -64,6 +64,10 @@ constexpr int kMoeMaxTiles = 32768;  // (expert, 128 rows of I) tiles of the gat
 constexpr int kMoeMaxShares = 4;  // K shares of a logit
 constexpr int kMoeSplitUnits = 8;  // gate / up units per CTA from which the experts go in two groups
 constexpr int kMoeWarps = kThreads / 32;
+// Experts of a CTA's gate / up run, one for each epilogue warp: as long as there are at
+// most three experts in use a CTA, a run is as long as three experts at most, and meets
+// four (the host refuses more; 256 experts need 86 SMs).
+constexpr int kMoeRunExperts = kEpiThreads / 32;
 
 struct MoeParams {
     CUtensorMap tmGU, tmGUE;  // gate and up weights of all experts: values, metadata
@@ -121,7 +125,7 @@ struct MoeShared {
     uint16_t list[kMoeMaxExperts];               // experts in use, in increasing order
     uint8_t slot[kMoeMaxExperts];                // an expert's place there
     float xscale[kMoeMaxTokens];
-    uint32_t hmax[4][kMoeMaxTokens];             // int8: largest |h| (bits) in this CTA's rows, its run's first experts
+    uint32_t hmax[kMoeRunExperts][kMoeMaxTokens];  // int8: largest |h| (bits) in this CTA's rows, its run's experts
     uint32_t red[kMoeWarps][8];
     uint32_t top[kMoeMaxTokens];
     uint32_t tmem, base, epoch, n_active, last, dead;
@@ -447,16 +451,14 @@ __device__ __forceinline__ uint32_t moe_add(uint32_t a, uint32_t b) {
     return I8 ? a + b : __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
 }
 
-// int8: one warp's largest |h| of a token, to shared memory for the first four
-// experts of the CTA's run: global atomics stall behind a full weight stream
-// (0.5 us each), so there is one per token and expert, at the end of the run.
-__device__ __forceinline__ void moe_note_max(const MoeParams& p, MoeShared& sh, int slot, int nth, int t, float h) {
+// int8: one warp's largest |h| of a token, to shared memory, for the CTA's run's
+// nth expert (kMoeRunExperts of them at most): global atomics stall behind a full
+// weight stream (0.5 us each), so there is one per token and expert, at the end of
+// the run.
+__device__ __forceinline__ void moe_note_max(MoeShared& sh, int nth, int t, float h) {
     // bits order as magnitudes, NaN above all
     const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(h) & 0x7fffffffu);
-    if ((threadIdx.x & 31u) == 0u) {
-        if (nth < 4) atomicMax(&sh.hmax[nth][t], m);
-        else atomicMax(p.amax + slot * kMoeMaxTokens + t, m);
-    }
+    if ((threadIdx.x & 31u) == 0u) atomicMax(&sh.hmax[nth][t], m);
 }
 
 // Two 64-bit words {value, tag, value, tag}: each word is read as it was
@@ -1000,7 +1002,7 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
                                                    int8_value((int)v[N_TILE + t], us, xs)
                                              : 0.f;
                         if (live) __stcg(p.h32 + ((size_t)slot * p.T + t) * p.I + r, h);
-                        moe_note_max(p, sh, slot, slot - slot0, t, h);
+                        moe_note_max(sh, slot - slot0, t, h);
                     }
                 } else if (live) {
 #pragma unroll
@@ -1075,7 +1077,7 @@ __global__ void __launch_bounds__(kThreads, 1) spmm24_moe_kernel(const __grid_co
                                     h[i] = moe_activate(int8_value((int)gv, gs, xs), p.act) * int8_value((int)uv, us, xs);
                                     __stcg(p.h32 + ((size_t)slot * p.T + tok) * p.I + r, h[i]);
                                 }
-                                moe_note_max(p, sh, slot, slot - slot0, tok, h[i]);
+                                moe_note_max(sh, slot - slot0, tok, h[i]);
                             } else {
                                 h[i] = moe_activate(__uint_as_float(gv), p.act) * __uint_as_float(uv);
                             }
