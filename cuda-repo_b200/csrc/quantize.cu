@@ -226,12 +226,12 @@ extern "C" cudaError_t spmm24_quantize_int8(cudaStream_t stream, const void* x, 
         if (((uintptr_t)x & 15u) || ((uintptr_t)q & 7u))
             return record_invalid("packed rows: x must be 16-byte and q 8-byte aligned");
         // CTAs per strip: eight where strips are few (64 elements a thread are 1.2
-        // us of arithmetic when one CTA has 4096 columns) or long (registers hold
-        // 4096 columns a CTA): 16 x 4096 5.4 us with one, 3.4 with eight; 509 x 4096
-        // 5.4 and 4.5; 4096 x 4096 15.1 and 20; 4096 x 11008 48 and 41.
+        // us of arithmetic when one CTA has 4096 columns; up to eight CTAs an SM) or long
+        // (registers hold 4096 columns a CTA): 16 x 4096 5.4 us with one, 3.4 with eight;
+        // 509 x 4096 5.4 and 4.5; 4096 x 4096 15.1 and 20; 4096 x 11008 48 and 41.
         const long long strips = ((long long)rows + 7) / 8;
         unsigned ctas = kMaxStripCtas;
-        while (ctas > 1 && cols <= 4096 && (strips * ctas > 8 * 148 || groups < 64 * (int)ctas)) ctas /= 2;
+        while (ctas > 1 && cols <= 4096 && (strips * ctas > 8LL * current_sms() || groups < 64 * (int)ctas)) ctas /= 2;
         const int each = (groups + (int)ctas - 1) / (int)ctas;
         const unsigned threads = (unsigned)(each < 512 ? (each + 31) / 32 * 32 : 512);
         if (strips * ctas > 0x7fffffffLL) return record_invalid("packed rows: too many rows");

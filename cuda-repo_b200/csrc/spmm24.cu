@@ -1779,14 +1779,13 @@ extern "C" cudaError_t spmm24_ipc_close(void* dev_ptr) {
 extern "C" size_t spmm24_workspace_bytes(int, int, int, int) { return 0; }
 
 namespace spmm24 {
-namespace {
 int current_sms() {
     int dev = 0;
-    int sms = (cudaGetDevice(&dev) == cudaSuccess) ? sm_count(dev) : 148;
-    if (sms <= 0) sms = 148;
+    if (cudaGetDevice(&dev) == cudaSuccess) return sm_count(dev);
     cudaGetLastError();
-    return sms;
+    return 148;
 }
+namespace {
 void fill_config(const Plan& pl, int stage_k, spmm24_config* out);
 }  // namespace
 }  // namespace spmm24

@@ -8,4 +8,6 @@ namespace spmm24 {
 cudaError_t record_invalid(const char* why);
 // Clears the calling thread's spmm24_last_error().
 void clear_last_error();
+// SMs of the current device (148 if there is none).
+int current_sms();
 }  // namespace spmm24
