@@ -106,8 +106,9 @@ __global__ void __launch_bounds__(512, 2) quantize_strips_kernel(const uint16_t*
     __shared__ RowScale rs[8];
     const int ctas = (int)ptx::cluster_nctarank(), rank = (int)ptx::cluster_ctarank();
     // "This CTA runs", awaited before the first store into another's shared
-    // memory: the loads pass meanwhile.
-    if (ctas > 1) ptx::cluster_arrive_release();
+    // memory; the loads pass meanwhile.  It orders no writes (a releasing arrival cost
+    // 3 of 41 us at 4096 x 11008).
+    if (ctas > 1) ptx::cluster_arrive_relaxed();
     ptx::grid_dep_wait();
     if (threadIdx.x == 0) ptx::grid_dep_launch();
     const int strip_id = (int)blockIdx.x / ctas, row0 = strip_id * 8;
@@ -227,8 +228,9 @@ extern "C" cudaError_t spmm24_quantize_int8(cudaStream_t stream, const void* x, 
             return record_invalid("packed rows: x must be 16-byte and q 8-byte aligned");
         // CTAs per strip: eight where strips are few (64 elements a thread are 1.2
         // us of arithmetic when one CTA has 4096 columns; up to eight CTAs an SM) or long
-        // (registers hold 4096 columns a CTA): 16 x 4096 5.4 us with one, 3.4 with eight;
-        // 509 x 4096 5.4 and 4.5; 4096 x 4096 15.1 and 20; 4096 x 11008 48 and 41.
+        // (registers hold 4096 columns a CTA), else as many as that leaves.  With 1, 2, 4
+        // and 8: 16 x 4096 5.9, 4.2, 3.4, 3.1 us; 509 x 4096 6.1, 4.4, 4.1, 4.3; 4096 x
+        // 4096 17.7, 16.2, 16.5, 18.9; 4096 x 11008 47, 48, 49, 41.
         const long long strips = ((long long)rows + 7) / 8;
         unsigned ctas = kMaxStripCtas;
         while (ctas > 1 && cols <= 4096 && (strips * ctas > 8LL * current_sms() || groups < 64 * (int)ctas)) ctas /= 2;
