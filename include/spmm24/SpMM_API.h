@@ -464,8 +464,9 @@ cudaError_t spmm24_launch_int8(cudaStream_t stream, const void* values, const vo
  *               (spmm24_device_status), zero it again.
  * flags: SPMM24_BF16, SPMM24_MOE_INT8; SPMM24_STATIC_WEIGHTS and SPMM24_NO_PDL
  * are accepted and change nothing (the kernel is launched cooperatively, in
- * stream order).  y and the workspace overlap no other operand.  Allocates
- * nothing.  Asynchronous on `stream`. */
+ * stream order).  The epilogue's residual may be y itself (one layout: each
+ * element is read by the thread that writes it); otherwise y and the workspace
+ * overlap no operand.  Allocates nothing.  Asynchronous on `stream`. */
 enum { SPMM24_MOE_INT8 = 32u };
 typedef struct spmm24_moe_layer {
     int tokens, hidden, inter, experts, top_k;
