@@ -9,16 +9,18 @@
 // 4096 K.  Here a pair walks tiles, the ring of loads runs on across them, and
 // eight warps of each CTA do nothing but epilogues.  TMEM is full (two
 // accumulators of 224 columns and the metadata), so the next tile's MMAs wait
-// until an accumulator has been read: eight epilogue warps take it to registers
-// at once, 112 columns of a row for each thread, release TMEM, and only then
-// scale, activate, round and store, while the next tile is multiplied.  Its first
-// half starts on the stages at hand while the second half is still being read.
+// until an accumulator has been read: eight epilogue warps take one to registers
+// at once, 112 columns of a row for each thread, release it, and only then scale,
+// activate, round and store.  The two follow one another: the next tile's first half
+// starts on the stages at hand while the first accumulator's values are stored, its
+// second half waits until they are and the second accumulator has been read.
 //
 // Measured: 11008 x 4096 x 4096 (418 tiles, 6 rounds of 74 pairs) 119.5 -> 99 us,
 // 8192^3 248 -> 230.  A stage takes 1160 cycles, what the tensor cores' operand
 // reads take at 128 bytes a cycle (A 4 KB, B 14 KB a step, eight steps); a tile
-// adds 9000: the drain of both accumulators that the head start does not cover,
-// and waits for loads (60 bytes a cycle and SM out of L2).
+// of 16 stages takes 27.7 thousand: 5.2 of them wait for the accumulators (the store
+// of the first that the head start does not cover) and 3.6 for loads (60 bytes a cycle
+// and SM out of L2).
 //
 // Row-major C needs N % 8 == 0 and 16-byte alignment, a packed C nothing.  No
 // residual.
