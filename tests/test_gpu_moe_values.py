@@ -6,7 +6,7 @@ import pytest
 
 import spmm24
 from act_values import act_tails
-from test_gpu_moe import Layer, _strips
+from test_gpu_moe import Layer, _matrix, _strips
 
 pytestmark = pytest.mark.gpu
 
@@ -213,3 +213,59 @@ def test_many_tokens_in_two_groups(cuda_device, shape, kind):
     ref, bound = L.reference(x, ids2.long(), w2)
     r = res[:T].T.double()
     L.check(L.result(out, T, True), ref + r, bound + 2.0 ** -22 * (ref.abs() + r.abs()))
+
+
+@pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
+def test_captured_decode_steps_take_turns_with_one_workspace(cuda_device, int8):
+    """Quantiser, int8 projection into strips, expert layer with the strips for residual, quantiser of its strips:
+    captured for two layers of different sizes that share a workspace, replayed in turn on new tokens, each step with
+    the bits of its own eager run."""
+    import torch
+
+    st = torch.cuda.Stream(cuda_device)
+    dt, steps = torch.bfloat16, []
+    sizes = [(5, 512, 384, 8, 2), (20, 1024, 640, 6, 2)]
+    layers = [Layer(cuda_device, H, inter, E, bf16=True, int8=int8, seed=n) for n, (T, H, inter, E, k) in enumerate(sizes)]
+    shared = torch.zeros(max(L.workspace(T, k).numel() for L, (T, _, _, _, k) in zip(layers, sizes)), dtype=torch.uint8,
+                         device=cuda_device)
+    for L, (T, H, inter, E, k) in zip(layers, sizes):
+        w, vals, meta, scale = _matrix(L.g, H, H, dt, True, False, cuda_device)
+        strips = (T + 7) // 8
+        b = dict(x=L.tokens(T), q=torch.empty(T, H, dtype=torch.int8, device=cuda_device), s=torch.empty(T, device=cuda_device),
+                 a=torch.zeros(strips * 8 * H, dtype=dt, device=cuda_device), y=torch.zeros(strips * 8 * H, dtype=dt, device=cuda_device),
+                 q2=torch.empty(T, H, dtype=torch.int8, device=cuda_device), s2=torch.empty(T, device=cuda_device))
+
+        def step(ws, L=L, T=T, H=H, k=k, b=b, vals=vals, meta=meta, scale=scale):
+            s = torch.cuda.current_stream(cuda_device)
+            spmm24.quantize_int8(b["x"], T, H, b["q"], b["s"], bf16=True)
+            assert spmm24.launch_int8(s, vals, b["q"], meta, b["a"], H, T, H, w_scale=scale, x_scale=b["s"], flags=spmm24.BF16,
+                                      alpha=4.0, out_layout=spmm24.OUT_PACKED_B) == 0
+            _, ids, w = L.run(b["x"], k, ws, y=b["y"], x_packed=b["a"], residual=b["a"], packed=True, stream=s)
+            spmm24.quantize_int8(b["y"], T, H, b["q2"], b["s2"], bf16=True, packed=True)
+            return ids, w
+
+        steps.append((step, b, L.workspace(T, k)))
+    inputs = [[torch.randn_like(b["x"].float()).to(dt) for _ in range(3)] for _, b, _ in steps]
+    want, graphs = [], []
+    with torch.cuda.stream(st):
+        for (step, b, own), xs in zip(steps, inputs):
+            want.append([])
+            for x in xs:
+                b["x"].copy_(x)
+                ids, w = step(own)
+                want[-1].append([ids.clone(), w.clone()] + [b[n].clone() for n in ("a", "y", "q2", "s2")])
+        st.synchronize()
+        for step, b, _ in steps:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=st):
+                out = step(shared)
+            graphs.append((g, out))
+        for i in range(3):
+            for (step, b, _), (g, out), xs, ref in zip(steps, graphs, inputs, want):
+                b["x"].copy_(xs[i])
+                for _ in range(4):
+                    g.replay()
+                for got, r in zip(list(out) + [b[n] for n in ("a", "y", "q2", "s2")], ref[i]):
+                    assert torch.equal(got, r)
+    torch.cuda.synchronize(cuda_device)
+    assert spmm24.device_status(0) == 0
