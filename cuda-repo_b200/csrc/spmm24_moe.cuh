@@ -41,9 +41,9 @@
 // stops, the others then give up in turn, TMEM is freed.
 //
 // Measured, E = 8, k = 2, 4096 x 11008: 1 token fp16 61 us (304 MB, 5.0 TB/s;
-// floor 46.5 at the copy rate), int8 53 (169 MB, 3.2; 25.8), 32 tokens int8 140
+// floor 46.5 at the copy rate), int8 54 (169 MB, 3.1; 25.8), 32 tokens int8 140
 // (676 MB, 4.8; 103); E = 64, k = 8, 2048 x 1024, 8 tokens bf16 70 (297 MB, 4.2;
-// 45.4); E = 5, k = 2, 1024 x 640, 3 tokens 18 (latency).  The weight stream runs
+// 45.4); E = 5, k = 2, 1024 x 640, 3 tokens 19 (latency).  The weight stream runs
 // at 6.0 TB/s; the rest is the front (routing known after 5 us, int8 6, of many
 // experts 8, and a first load of 2), the int8 rows' barriers where a group's stream is
 // too short to hide them (a message through L2 takes 1-2 us while it is full),
